@@ -20,6 +20,10 @@
 #include "comm.h"
 #include "cpu_ref.h"
 
+namespace sqstep {
+void register_step(pybind11::module& m);  // step_bindings.cpp
+}
+
 namespace {
 
 #define CHECK_CUDA(x) TORCH_CHECK((x).is_cuda(), #x " must be a CUDA tensor")
@@ -1285,6 +1289,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pq_adc", &pq_adc_cuda);
   m.def("hadamard_rows", &hadamard_rows_cuda, py::arg("x"), py::arg("signs"), py::arg("block"),
         py::arg("out") = py::none());
+  sqstep::register_step(m);
   sqcpu::register_cpu(m);
   sqhost::register_host(m);
   sqgram::register_grammar(m);

@@ -15,3 +15,15 @@ from .kernels import (  # noqa: F401
     w4a16_linear,
     workspace,
 )
+from .step import (  # noqa: F401
+    LoraPlan,
+    LoraPool,
+    StepLayout,
+    fuse_lora,
+    lora_add,
+    lora_linear,
+    lora_plan,
+    moe_route_scored,
+    sample_uniform,
+    step_layout,
+)
