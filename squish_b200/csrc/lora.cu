@@ -128,8 +128,7 @@ constexpr int kWarps = kThreads / 32;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -139,14 +138,72 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 __device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }
+// silu(g) * u with the hardware's exponential and reciprocal (2 and 1 ulp). Below g = -87 the
+// reciprocal is flushed to 0; the product it replaces is smaller than 1.1e-36 |u|.
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * g));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * r * u;
+}
+// y added to the accumulators of 16 rows x 32 columns: a lane's 8 columns of its two rows ...
+__device__ __forceinline__ void add_to(float (&acc)[4][4], uint4 y0, uint4 y1) {
+  const uint32_t w0[4] = {y0.x, y0.y, y0.z, y0.w}, w1[4] = {y1.x, y1.y, y1.z, y1.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    acc[j][0] += lo_f(w0[j]);
+    acc[j][1] += hi_f(w0[j]);
+    acc[j][2] += lo_f(w1[j]);
+    acc[j][3] += hi_f(w1[j]);
+  }
+}
+// ... or as their start, where y is at hand before the products (16 additions and 16 zeros fewer).
+__device__ __forceinline__ void start_from(float (&acc)[4][4], uint4 y0, uint4 y1) {
+  const uint32_t w0[4] = {y0.x, y0.y, y0.z, y0.w}, w1[4] = {y1.x, y1.y, y1.z, y1.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t a = w0[j], b = w1[j];
+    acc[j][0] = lo_f(a);
+    acc[j][1] = hi_f(a);
+    acc[j][2] = lo_f(b);
+    acc[j][3] = hi_f(b);
+  }
+}
+// A lane's 8 output columns of row r (0, 1), rounded once.
+template <bool SILU, int G>
+__device__ __forceinline__ uint4 finish(const float (&acc)[G][4][4], int r) {
+  uint32_t o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = acc[0][j][2 * r], b = acc[0][j][2 * r + 1];
+    o[j] = SILU ? pack_bf16(silu_mul(a, acc[G - 1][j][2 * r]), silu_mul(b, acc[G - 1][j][2 * r + 1])) : pack_bf16(a, b);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
 
-// R: padded rank of the pool; RW: warps along the rows of a tile (16 rows each).
-template <int R, int RW, bool SILU>
-__global__ void __launch_bounds__(kThreads) lora_add_kernel(const LoraParams p) {
+// One rank step of the expand for 16 rows x 32 columns: the lower part of h, then the upper. The four
+// tiles' products alternate, so that no product waits for the one before it.
+template <int R>
+__device__ __forceinline__ void expand_step(float (&acc)[4][4], const uint4 (&lo)[2], const uint4 (&hi)[2],
+                                            const uint4 (&w)[4]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint4 a0 = h ? hi[0] : lo[0], a1 = h ? hi[1] : lo[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mma16816(acc[j], a0.x, a1.x, a0.y, a1.y, w[j].x, w[j].y);
+    if (R != 16) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mma16816(acc[j], a0.z, a1.z, a0.w, a1.w, w[j].z, w[j].w);
+    }
+  }
+}
+
+// Tiles of 16 rows (decode). R: padded rank of the pool.
+template <int R, bool SILU>
+__global__ void __launch_bounds__(kThreads) lora_row16_kernel(const LoraParams p) {
   constexpr int RT = R / 8;           // 8-wide rank tiles
-  constexpr int KW = kWarps / RW;     // warps along K (shrink) / along the columns (expand)
-  constexpr int ROWS = RW * 16;
+  constexpr int KW = kWarps;          // the warps split K (shrink), then the columns (expand)
+  constexpr int ROWS = 16;
   constexpr int PS = R + 4;           // row stride of the fp32 shares (4: rows on distinct banks)
   constexpr int HS = R + 8;           // row stride of the bf16 parts of h
   pdl_wait();
@@ -164,10 +221,10 @@ __global__ void __launch_bounds__(kThreads) lora_add_kernel(const LoraParams p) 
   const int C = gridDim.z, cr = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int rw = warp % RW, kw = warp / RW;
+  const int kw = warp;
   if (tid < ROWS) rows[tid] = tid < cnt ? p.order[tile.y + tid] : -1;
   __syncthreads();
-  const int row0 = rows[rw * 16 + g], row1 = rows[rw * 16 + g + 8];
+  const int row0 = rows[g], row1 = rows[g + 8];
   const int live = min(R, (rank + 15) / 16 * 16);  // ranks computed: whole 16-wide steps
 
   if (rank > 0) {
@@ -204,7 +261,7 @@ __global__ void __launch_bounds__(kThreads) lora_add_kernel(const LoraParams p) 
         }
       }
     }
-    float* pw = part + ((size_t)kw * ROWS + rw * 16) * PS;
+    float* pw = part + (size_t)kw * ROWS * PS;
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       if (i * 8 >= live) break;
@@ -263,7 +320,7 @@ __global__ void __launch_bounds__(kThreads) lora_add_kernel(const LoraParams p) 
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const __nv_bfloat16* src = hh + (size_t)(q * ROWS + rw * 16 + g + 8 * r) * HS;
+          const __nv_bfloat16* src = hh + (size_t)(q * ROWS + g + 8 * r) * HS;
           if (R == 16) {
             const uint2 v = *reinterpret_cast<const uint2*>(src + t * 4);
             fa[q][ks][r] = make_uint4(v.x, v.y, 0, 0);
@@ -278,8 +335,8 @@ __global__ void __launch_bounds__(kThreads) lora_add_kernel(const LoraParams p) 
   const int units = SILU ? p.N / 64 : (p.N + 31) / 32;
   const int u0 = (int)((long long)units * cr / C), u1 = (int)((long long)units * (cr + 1) / C);
   for (int u = u0 + kw; u < u1; u += KW) {
-    uint4 yv[G][2];
     float acc[G][4][4];
+    uint4 yv[G][2];  // loaded first, added last: the products do not wait for it
 #pragma unroll
     for (int q = 0; q < G; ++q) {
       // first of the 32 columns of y / B: plain, or the gate / up half of block u / 2
@@ -291,71 +348,288 @@ __global__ void __launch_bounds__(kThreads) lora_add_kernel(const LoraParams p) 
       for (int j = 0; j < 4; ++j) acc[q][j][0] = acc[q][j][1] = acc[q][j][2] = acc[q][j][3] = 0.f;
       if (rank > 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int n = col + (g >> 1) * 8 + 2 * j + (g & 1);  // (g, j) -> column: a lane's 4 tiles are 8 columns
+        for (int ks = 0; ks < KS; ++ks) {
+          if (R != 16 && ks * 32 >= live) break;
+          uint4 w[4];
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            if (R != 16 && ks * 32 >= live) break;
-            uint4 w = make_uint4(0, 0, 0, 0);
+          for (int j = 0; j < 4; ++j) {
+            const int n = col + (g >> 1) * 8 + 2 * j + (g & 1);  // (g, j) -> column: a lane's 4 tiles are 8 columns
+            w[j] = make_uint4(0, 0, 0, 0);
             if (SILU || n < p.N) {
               if (R == 16) {
                 const uint2 v = __ldg(reinterpret_cast<const uint2*>(bs + (size_t)n * R + t * 4));
-                w.x = v.x;
-                w.y = v.y;
+                w[j].x = v.x;
+                w[j].y = v.y;
               } else {
-                w = __ldg(reinterpret_cast<const uint4*>(bs + (size_t)n * R + ks * 32 + t * 8));
+                w[j] = __ldg(reinterpret_cast<const uint4*>(bs + (size_t)n * R + ks * 32 + t * 8));
               }
             }
-#pragma unroll
-            for (int h = 1; h >= 0; --h) {  // lower part first
-              mma16816(acc[q][j], fa[h][ks][0].x, fa[h][ks][1].x, fa[h][ks][0].y, fa[h][ks][1].y, w.x, w.y);
-              if (R != 16) mma16816(acc[q][j], fa[h][ks][0].z, fa[h][ks][1].z, fa[h][ks][0].w, fa[h][ks][1].w, w.z, w.w);
-            }
           }
+          expand_step<R>(acc[q], fa[1][ks], fa[0][ks], w);
         }
       }
     }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = r ? row1 : row0;
-      if (row < 0) continue;
-      uint32_t o[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t yw = reinterpret_cast<const uint32_t*>(&yv[0][r])[j];
-        float a = lo_f(yw) + acc[0][j][2 * r], b = hi_f(yw) + acc[0][j][2 * r + 1];
-        if (SILU) {
-          const uint32_t uw = reinterpret_cast<const uint32_t*>(&yv[G - 1][r])[j];
-          a = silu_mul(a, lo_f(uw) + acc[G - 1][j][2 * r]);
-          b = silu_mul(b, hi_f(uw) + acc[G - 1][j][2 * r + 1]);
-        }
-        o[j] = pack_bf16(a, b);
-      }
-      const int oc = u * 32 + t * 8;
-      if (SILU || oc < p.N)
-        *reinterpret_cast<uint4*>(p.out + row * p.ldo + oc) = make_uint4(o[0], o[1], o[2], o[3]);
+    for (int q = 0; q < G; ++q) add_to(acc[q], yv[q][0], yv[q][1]);
+    const int oc = u * 32 + t * 8;
+    if (SILU || oc < p.N) {
+      if (row0 >= 0) *reinterpret_cast<uint4*>(p.out + row0 * p.ldo + oc) = finish<SILU, G>(acc, 0);
+      if (row1 >= 0) *reinterpret_cast<uint4*>(p.out + row1 * p.ldo + oc) = finish<SILU, G>(acc, 1);
     }
   }
   if (rank > 0) cl.sync();  // peers may still read this CTA's share
 }
 
-template <int R, int RW, bool SILU>
+// ---------------------------------------------------------------- tiles of 64 rows (prefill)
+__device__ __forceinline__ void cp16(void* dst, const void* src, bool on) {  // 16 bytes, or zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Offset of 16-byte chunk c (0..7) of row r in a tile of 128-byte rows. A fragment load reads four
+// chunks of two neighbouring rows per phase: odd rows swap their halves, so they meet no bank twice.
+__device__ __forceinline__ int sw(int r, int c) { return r * 128 + ((c ^ ((r & 1) << 2)) << 4); }
+
+// 8 warps: 4 row groups of 16 x 2 halves (of the rank tiles in the shrink, of the columns in the
+// expand). One ring of stages runs through both products: x and A in 64-wide steps of K, then y and
+// B in units of 64 columns (gate and up: 128), so the first units of y are in flight while the
+// cluster exchanges h. The loads are what bounds it: without the ring each warp waited for its own
+// fragments (8185 rows, K 4096, N 6144, rank 64: 240 us, 1.1 TB/s).
+template <int R, bool SILU>
+struct Tile64 {
+  static constexpr int G = SILU ? 2 : 1;
+  static constexpr int kStage = G * 64 * 128 + G * 64 * R * 2 > 64 * 128 + R * 128 ? G * 64 * 128 + G * 64 * R * 2
+                                                                                  : 64 * 128 + R * 128;
+  static constexpr int kPart = 64 * (R + 4) * 4, kH = 2 * 64 * (R + 8) * 2;
+  // as many stages as two resident CTAs leave room for, at least two
+  static constexpr int kFit = (113 * 1024 - kPart - kH - 1024) / kStage;
+  static constexpr int S = kFit > 5 ? 5 : kFit < 2 ? 2 : kFit;
+  static constexpr int kSmem = S * kStage + kPart + kH;
+};
+
+template <int R, bool SILU>
+__global__ void __launch_bounds__(kThreads) lora_row64_kernel(const LoraParams p) {
+  using TC = Tile64<R, SILU>;
+  constexpr int S = TC::S, G = TC::G;
+  constexpr int RH = R / 16;        // 8-wide rank tiles of a warp: 2 i + half
+  constexpr int PS = R + 4, HS = R + 8;
+  pdl_wait();
+  pdl_trigger();
+  if ((int)blockIdx.x >= *p.num_tiles) return;  // the whole cluster
+  const int4 tile = p.tiles[blockIdx.x];
+  const int slot = tile.x, cnt = tile.z;
+  const int rank = slot >= 0 ? p.rank[slot] : 0;
+  if (rank <= 0 && p.in_place) return;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* part = reinterpret_cast<float*>(smem + S * TC::kStage);                         // [64][PS]
+  __nv_bfloat16* hh = reinterpret_cast<__nv_bfloat16*>(smem + S * TC::kStage + TC::kPart);  // [2][64][HS]
+  __shared__ int rows[64];
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = gridDim.z, cr = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int rw = warp >> 1, hf = warp & 1;
+  if (tid < 64) rows[tid] = tid < cnt ? p.order[tile.y + tid] : -1;
+  __syncthreads();
+  const int live = min(R, (rank + 15) / 16 * 16);
+  const int steps = rank > 0 ? (p.K + 63) / 64 : 0;
+  const int k0 = (int)((long long)steps * cr / C), n1 = (int)((long long)steps * (cr + 1) / C) - k0;
+  const int units = (p.N + 64 * G - 1) / (64 * G);
+  const int u0 = (int)((long long)units * cr / C), n2 = (int)((long long)units * (cr + 1) / C) - u0;
+  const __nv_bfloat16* as = p.a + (size_t)(slot < 0 ? 0 : slot) * R * p.K;
+  const __nv_bfloat16* bs = p.b + (size_t)(slot < 0 ? 0 : slot) * p.N * R;
+
+  // a thread copies chunk tid % 8 of rows tid / 8 and tid / 8 + 32 of a 64-row tile
+  const int lr = tid >> 3, lc = tid & 7;
+  const int ra = rows[lr], rb = rows[lr + 32];
+  const __nv_bfloat16* xa = p.x + (ra < 0 ? 0 : ra) * p.ldx + lc * 8;
+  const __nv_bfloat16* xb = p.x + (rb < 0 ? 0 : rb) * p.ldx + lc * 8;
+  const __nv_bfloat16* ya = p.y + (ra < 0 ? 0 : ra) * p.ldy + lc * 8;
+  const __nv_bfloat16* yb = p.y + (rb < 0 ? 0 : rb) * p.ldy + lc * 8;
+  int wr = 0, rd = 0;  // offsets of the next stage to fill and to use
+  auto next = [](int& at) { at = at == (S - 1) * TC::kStage ? 0 : at + TC::kStage; };
+  auto issue = [&](int i) {
+    uint8_t* st = smem + wr;
+    next(wr);
+    if (i < n1) {
+      const int k = (k0 + i) * 64;
+      const bool in = k + lc * 8 < p.K;
+      cp16(st + sw(lr, lc), in ? xa + k : p.x, in && ra >= 0);
+      cp16(st + sw(lr + 32, lc), in ? xb + k : p.x, in && rb >= 0);
+      uint8_t* sa = st + 64 * 128;
+#pragma unroll
+      for (int r = 0; r < R; r += 32)
+        if (r + lr < live) cp16(sa + sw(r + lr, lc), in ? as + (size_t)(r + lr) * p.K + k + lc * 8 : as, in);
+    } else if (i < n1 + n2) {
+      const int col = (u0 + i - n1) * 64 * G;
+#pragma unroll
+      for (int q = 0; q < G; ++q) {
+        const int c = col + q * 64;
+        const bool in = c + lc * 8 < p.N;
+        cp16(st + q * 8192 + sw(lr, lc), in ? ya + c : p.y, in && ra >= 0);
+        cp16(st + q * 8192 + sw(lr + 32, lc), in ? yb + c : p.y, in && rb >= 0);
+      }
+      uint8_t* sb = st + G * 8192;
+      constexpr int CH = R / 8;  // 16-byte pieces of a B row
+      const int c = tid % CH;
+      if (c * 8 < live) {
+#pragma unroll
+        for (int n = tid / CH; n < G * 64; n += kThreads / CH) {
+          const bool in = col + n < p.N;
+          const __nv_bfloat16* src = in ? bs + (size_t)(col + n) * R + c * 8 : bs;
+          if (R >= 64) cp16(sb + (c >> 3) * (G * 64 * 128) + sw(n, c & 7), src, in);
+          else cp16(sb + n * R * 2 + c * 16, src, in);
+        }
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) issue(i);
+
+  // ---- shrink
+  if (rank > 0) {
+    float acc[RH][4];
+#pragma unroll
+    for (int i = 0; i < RH; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    for (int i = 0; i < n1; ++i) {
+      cp_wait<S - 2>();
+      __syncthreads();
+      issue(i + S - 1);
+      const uint8_t* st = smem + rd;
+      next(rd);
+      const uint8_t* sa = st + 64 * 128;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 v0 = *reinterpret_cast<const uint4*>(st + sw(rw * 16 + g, h * 4 + t));
+        const uint4 v1 = *reinterpret_cast<const uint4*>(st + sw(rw * 16 + g + 8, h * 4 + t));
+        uint4 w[RH];
+#pragma unroll
+        for (int j = 0; j < RH; ++j)
+          if ((2 * j + hf) * 8 < live) w[j] = *reinterpret_cast<const uint4*>(sa + sw((2 * j + hf) * 8 + g, h * 4 + t));
+#pragma unroll
+        for (int j = 0; j < RH; ++j)
+          if ((2 * j + hf) * 8 < live) mma16816(acc[j], v0.x, v1.x, v0.y, v1.y, w[j].x, w[j].y);
+#pragma unroll
+        for (int j = 0; j < RH; ++j)
+          if ((2 * j + hf) * 8 < live) mma16816(acc[j], v0.z, v1.z, v0.w, v1.w, w[j].z, w[j].w);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < RH; ++j) {
+      const int c = (2 * j + hf) * 8 + 2 * t;
+      if ((2 * j + hf) * 8 >= live) break;
+      *reinterpret_cast<float2*>(part + (rw * 16 + g) * PS + c) = make_float2(acc[j][0], acc[j][1]);
+      *reinterpret_cast<float2*>(part + (rw * 16 + g + 8) * PS + c) = make_float2(acc[j][2], acc[j][3]);
+    }
+    cl.sync();
+    const float sc = p.scale[slot];
+    const int nv = live / 4;
+    for (int i = tid; i < 64 * nv; i += kThreads) {
+      const int r = i / nv, c = (i - r * nv) * 4;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q = 0; q < C; ++q) {
+        const float4 v = *reinterpret_cast<const float4*>(cl.map_shared_rank(part, q) + r * PS + c);
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+      }
+      s.x *= sc;
+      s.y *= sc;
+      s.z *= sc;
+      s.w *= sc;
+      const uint32_t h01 = pack_bf16(s.x, s.y), h23 = pack_bf16(s.z, s.w);
+      *reinterpret_cast<uint2*>(hh + r * HS + c) = make_uint2(h01, h23);
+      *reinterpret_cast<uint2*>(hh + (64 + r) * HS + c) =
+          make_uint2(pack_bf16(s.x - lo_f(h01), s.y - hi_f(h01)), pack_bf16(s.z - lo_f(h23), s.w - hi_f(h23)));
+    }
+    __syncthreads();
+  }
+
+  // ---- expand
+  constexpr int KS = R == 16 ? 1 : R / 32;
+  uint4 fa[2][KS][2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const __nv_bfloat16* src = hh + (q * 64 + rw * 16 + g + 8 * r) * HS;
+        fa[q][ks][r] = make_uint4(0, 0, 0, 0);
+        if (R == 16) {
+          if (rank > 0) {
+            const uint2 v = *reinterpret_cast<const uint2*>(src + t * 4);
+            fa[q][ks][r].x = v.x;
+            fa[q][ks][r].y = v.y;
+          }
+        } else if (ks * 32 + t * 8 < live) {
+          fa[q][ks][r] = *reinterpret_cast<const uint4*>(src + ks * 32 + t * 8);
+        }
+      }
+  const int row0 = rows[rw * 16 + g], row1 = rows[rw * 16 + g + 8];
+  for (int i = n1; i < n1 + n2; ++i) {
+    cp_wait<S - 2>();
+    __syncthreads();
+    issue(i + S - 1);
+    const uint8_t* st = smem + rd;
+    next(rd);
+    const uint8_t* sb = st + G * 8192;
+    float acc[G][4][4];
+#pragma unroll
+    for (int q = 0; q < G; ++q) {
+      start_from(acc[q], *reinterpret_cast<const uint4*>(st + q * 8192 + sw(rw * 16 + g, hf * 4 + t)),
+                 *reinterpret_cast<const uint4*>(st + q * 8192 + sw(rw * 16 + g + 8, hf * 4 + t)));
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks * 32 >= live) break;
+        uint4 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int n = q * 64 + hf * 32 + (g >> 1) * 8 + 2 * j + (g & 1);
+          w[j] = make_uint4(0, 0, 0, 0);
+          if (R == 16) {
+            const uint2 v = *reinterpret_cast<const uint2*>(sb + n * R * 2 + t * 8);
+            w[j].x = v.x;
+            w[j].y = v.y;
+          } else if (ks * 32 + t * 8 < live) {
+            if (R >= 64) w[j] = *reinterpret_cast<const uint4*>(sb + (ks >> 1) * (G * 64 * 128) + sw(n, (ks & 1) * 4 + t));
+            else w[j] = *reinterpret_cast<const uint4*>(sb + n * R * 2 + t * 16);
+          }
+        }
+        expand_step<R>(acc[q], fa[1][ks], fa[0][ks], w);
+      }
+    }
+    const int oc = (u0 + i - n1) * 64 + hf * 32 + t * 8;
+    if (SILU || oc < p.N) {
+      if (row0 >= 0) *reinterpret_cast<uint4*>(p.out + row0 * p.ldo + oc) = finish<SILU, G>(acc, 0);
+      if (row1 >= 0) *reinterpret_cast<uint4*>(p.out + row1 * p.ldo + oc) = finish<SILU, G>(acc, 1);
+    }
+  }
+  if (rank > 0) cl.sync();  // peers may still read this CTA's share
+}
+
+template <int R, bool SILU>
 cudaError_t launch_lora(const LoraParams& p, int C, cudaStream_t s) {
-  constexpr int ROWS = RW * 16, KW = kWarps / RW;
-  constexpr size_t smem = (size_t)KW * ROWS * (R + 4) * 4 + (size_t)2 * ROWS * (R + 8) * 2;
+  const bool small = p.tm == 16;
+  constexpr size_t smem16 = (size_t)kWarps * 16 * (R + 4) * 4 + (size_t)2 * 16 * (R + 8) * 2;
+  const size_t smem = small ? smem16 : (size_t)Tile64<R, SILU>::kSmem;
+  auto* kern = small ? lora_row16_kernel<R, SILU> : lora_row64_kernel<R, SILU>;
   if (smem > 48 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(lora_add_kernel<R, RW, SILU>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  SQ_LAUNCH((lora_add_kernel<R, RW, SILU>), dim3(p.max_tiles, 1, C), dim3(kThreads), smem, s, C, p);
+  SQ_LAUNCH(kern, dim3(p.max_tiles, 1, C), dim3(kThreads), smem, s, C, p);
   return cudaGetLastError();
 }
 
 template <int R>
 cudaError_t launch_rank(const LoraParams& p, int C, cudaStream_t s) {
-  if (p.tm == 16) return p.silu ? launch_lora<R, 1, true>(p, C, s) : launch_lora<R, 1, false>(p, C, s);
-  return p.silu ? launch_lora<R, 4, true>(p, C, s) : launch_lora<R, 4, false>(p, C, s);
+  return p.silu ? launch_lora<R, true>(p, C, s) : launch_lora<R, false>(p, C, s);
 }
 
 }  // namespace
@@ -377,6 +651,7 @@ cudaError_t lora_add_launch(const LoraParams& p, int num_sms, cudaStream_t s) {
   if (p.K % 8 || p.N % 8 || (p.silu && p.N % 128) || (p.tm != 16 && p.tm != 64)) return cudaErrorInvalidValue;
   int C = 8;
   while (C > 1 && p.max_tiles * C > 4 * num_sms) C >>= 1;
+  if (const char* e = getenv("LORA_C")) C = atoi(e);
   switch (p.R) {
     case 16: return launch_rank<16>(p, C, s);
     case 32: return launch_rank<32>(p, C, s);

@@ -108,11 +108,12 @@ def route_ref(logits, k, score="softmax", bias=None, groups=1, top_groups=None, 
 
 def lora_ref(x, y, rows, adapters, silu=False):
     """(out, bound) in float64: the exact result and the error that fp32 sums over K terms, h held
-    as two bf16 (2^-16 of it) and one rounding to bf16 (half a step: 2^-8 relative) may reach.
+    as two bf16 (2^-16 of it), a sum that starts from y (at most 16 steps of 16 ranks, each off by up
+    to 2^-23 of y: 2^-19 |y|) and one rounding to bf16 (half a step: 2^-8 relative) may reach.
     ``adapters``: {slot: (A, B, scale)}."""
     x64, out = x.double().cpu(), y.double().cpu().clone()
     K = x.shape[1]
-    slack = torch.zeros_like(out)
+    slack = out.abs() * 2.0**-19
     for s, (a, b, sc) in adapters.items():
         sel = (rows.cpu() == s).nonzero().flatten()
         if not sel.numel():
@@ -126,7 +127,9 @@ def lora_ref(x, y, rows, adapters, silu=False):
         g, u = out.view(m, n // 128, 2, 64).unbind(2)
         dg, du = slack.view(m, n // 128, 2, 64).unbind(2)
         sg = g * torch.sigmoid(g)
-        # |silu'| <= 1.1; the exponential and the divide are off by less than 2^-18 of the result
-        slack = 1.1 * dg * u.abs() + sg.abs() * du + dg * du + (sg * u).abs() * 2.0**-18
+        # |silu'| <= 1.1; the exponential's argument rounds by 2^-24 |g| log2 e and the exponential and
+        # reciprocal by 3 ulp: together below 2^-18 of the result for |g| <= 40; results below
+        # 1.1e-36 |u| may be flushed
+        slack = 1.1 * dg * u.abs() + sg.abs() * du + dg * du + (sg * u).abs() * 2.0**-18 + 1.1e-36 * u.abs()
         out, slack = (sg * u).reshape(m, n // 2), slack.reshape(m, n // 2)
     return out, out.abs() * 2.0**-8 + slack + 2.0**-126
