@@ -10,9 +10,10 @@
 // One warp per token, lane i holds the EPL consecutive experts from i * EPL on, so the lowest lane
 // among equals is the lowest index and a pick is one warp-wide integer max of order-preserving
 // keys plus a ballot. Without a bias the choice follows the logits themselves (both scores are
-// monotone in them): no rounding can reorder it. With a bias, or sums of two scores, c is compared
-// in fp32 with a known error bound; a row in which two compared values lie closer than twice the
-// bound is chosen again in fp64 by the same warp, so the ids are those of the exact scores.
+// monotone in them): no rounding can reorder it. With a bias, fp32 values cut the row to a short
+// list (with a margin for their error) whose exact values, one fp64 score per lane, are compared.
+// Group scores are compared in fp32; where the last open and the first closed group lie within the
+// error bound the same warp ranks the groups again in fp64. So the ids are those of the exact scores.
 #include "kernels.h"
 #include "launch.cuh"
 #include "step_ops.h"
@@ -27,7 +28,7 @@ constexpr float kNegInf = -INFINITY;
 
 __device__ __forceinline__ uint32_t ord32(float f) {
   const uint32_t u = __float_as_uint(f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float unord32(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
@@ -40,13 +41,27 @@ __device__ __forceinline__ double score64(float x, bool sigmoid, float m, double
   return (x == m ? 1.0 : exp((double)x - (double)m)) * inv_z;
 }
 
+// Scores for the fp32 choice: the hardware's exponential and reciprocal (2 and 1 ulp).
+__device__ __forceinline__ float exp_fast(float x) {  // x <= 0 or the score saturates: flushing is harmless
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(1.4426950408889634f * x));
+  return e;
+}
+__device__ __forceinline__ float sigmoid_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + exp_fast(-x)));
+  return r;
+}
+
+__device__ __forceinline__ float max2(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float min2(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double max2(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ double min2(double a, double b) { return fmin(a, b); }
 // The two largest of (a1 >= a2) and (b1 >= b2).
 template <class S>
 __device__ __forceinline__ void merge2(S& a1, S& a2, S b1, S b2) {
-  const S lo = a1 < b1 ? a1 : b1, hi = a1 < b1 ? b1 : a1;
-  const S s2 = a2 < b2 ? b2 : a2;
-  a1 = hi;
-  a2 = lo < s2 ? s2 : lo;
+  a2 = max2(min2(a1, b1), max2(a2, b2));
+  a1 = max2(a1, b1);
 }
 
 struct Shape {
@@ -62,7 +77,10 @@ __device__ __forceinline__ void group_top2(const S (&v)[EPL], const Shape& sh, i
   if (sh.lanes > 0) {
     S t1 = ninf, t2 = ninf;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) merge2(t1, t2, v[i], ninf);
+    for (int i = 0; i < EPL; ++i) {
+      t2 = max2(t2, min2(t1, v[i]));
+      t1 = max2(t1, v[i]);
+    }
     S r1 = t1, r2 = t2;
     const int base = lane / sh.lanes * sh.lanes;
     for (int o = 1; o < sh.lanes; ++o) {
@@ -85,55 +103,105 @@ __device__ __forceinline__ void group_top2(const S (&v)[EPL], const Shape& sh, i
   }
 }
 
-// fp32 choice. gscore: this lane's group score (lane < groups); c: choice values. Returns false
-// when two compared values lie within `tol` of each other (tol_g for groups; < 0: exact values).
-template <int EPL>
-__device__ __forceinline__ bool choose32(const float (&c)[EPL], float gscore, const Shape& sh, int lane, float tol_g,
-                                         float tol, int& my_id) {
-  bool sure = true;
-  unsigned open = kFull;
-  if (sh.groups > 1) {
-    uint32_t gk = lane < sh.groups ? ord32(clean(gscore)) : 0u;
-    open = 0;
-    float last = 0.f;
-    for (int g = 0; g < sh.top_groups; ++g) {
-      const uint32_t m = __reduce_max_sync(kFull, gk);
-      const int win = __ffs(__ballot_sync(kFull, gk == m)) - 1;
-      open |= 1u << win;
-      if (lane == win) gk = 0u;
-      last = unord32(m);
-    }
-    if (tol_g >= 0.f && sh.top_groups < sh.groups) {
-      const float next = unord32(__reduce_max_sync(kFull, gk));
-      if (!(last - next > tol_g * (1.f + fabsf(last)))) sure = false;
-    }
+// Open groups by score (lane g < groups: gscore). sure: false when the last open and the first closed
+// group lie within tol (1 + |score|) of each other; tol < 0: the scores are exact.
+__device__ __forceinline__ unsigned open_groups32(float gscore, const Shape& sh, int lane, float tol, bool& sure) {
+  uint32_t gk = lane < sh.groups ? ord32(clean(gscore)) : 0u;
+  unsigned open = 0;
+  uint32_t last = 0;
+  for (int g = 0; g < sh.top_groups; ++g) {
+    last = __reduce_max_sync(kFull, gk);
+    const int win = __ffs(__ballot_sync(kFull, gk == last)) - 1;
+    open |= 1u << win;
+    if (lane == win) gk = 0u;
   }
-  uint32_t k[EPL];
-  uint32_t best = 0u;
-  int bi = 0;
+  sure = true;
+  if (tol >= 0.f && sh.top_groups < sh.groups) {
+    const float a = unord32(last), b = unord32(__reduce_max_sync(kFull, gk));
+    sure = a - b > tol * (1.f + fabsf(a));
+  }
+  return open;
+}
+
+constexpr int kListK = 10;  // picks up to which the short list is used
+
+// Short list of a row: the K-th largest of the lanes' maxima is a bound that at least K values reach
+// and (for K <= 10) a few more; those down to `margin` below it are laid out in index order, one per
+// lane, where a pick is a maximum and a ballot. (Picking from 32 * EPL values costs every lane a new
+// maximum of its EPL values per pick.) Returns their number, or 33 when they are more than the lanes.
+template <int EPL>
+__device__ __forceinline__ int short_list(const uint32_t (&k)[EPL], int K, float margin, int lane, uint2* cand,
+                                          uint2& my) {
+  uint32_t lm = 0u, bound = 0u;
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane * EPL + i;
-    bool in = e < sh.E;
-    if (sh.groups > 1 && in) in = (open >> (sh.lanes > 0 ? lane / sh.lanes : e / sh.gsize)) & 1u;
-    k[i] = in ? ord32(c[i]) : 0u;
+  for (int i = 0; i < EPL; ++i) lm = max(lm, k[i]);
+  for (int kk = 0; kk < K; ++kk) {
+    bound = __reduce_max_sync(kFull, lm);
+    const int win = __ffs(__ballot_sync(kFull, lm == bound)) - 1;
+    if (lane == win) lm = 0u;
+  }
+  if (bound != 0u && margin > 0.f) {
+    const float v = unord32(bound);
+    bound = v > kNegInf ? ord32(v - margin * (1.f + fabsf(v))) : 1u;
+  }
+  bound = max(bound, 1u);  // (fewer open lanes than picks: every open value)
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) n += k[i] >= bound;
+  int at = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(kFull, at, o);
+    if (lane >= o) at += v;
+  }
+  const int total = __shfl_sync(kFull, at, 31);
+  if (total > 32) return 33;
+  at -= n;
+  if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (k[i] >= bound) cand[at++] = make_uint2(k[i], lane * EPL + i);
+  }
+  __syncwarp();
+  my = lane < total ? cand[lane] : make_uint2(0u, 0u);
+  return total;
+}
+
+// The K largest of 32 keys (hi, lo), in order; lane kk returns the id of pick kk.
+template <bool kTwo>
+__device__ __forceinline__ int pick_list(uint32_t hi, uint32_t lo, int id, int K, int lane) {
+  int my_id = 0;
+  for (int kk = 0; kk < K; ++kk) {
+    const uint32_t m = __reduce_max_sync(kFull, hi);
+    unsigned w = __ballot_sync(kFull, hi == m);
+    if (kTwo && (w & (w - 1u))) {  // the upper words tie: the lower ones decide
+      const uint32_t l = __reduce_max_sync(kFull, hi == m ? lo : 0u);
+      w &= __ballot_sync(kFull, lo == l);
+    }
+    const int win = __ffs(w) - 1;
+    const int picked = __shfl_sync(kFull, id, win);
+    if (lane == kk) my_id = picked;
+    if (lane == win) hi = 0u;
+  }
+  return my_id;
+}
+
+// The K largest of all keys, one after another (more picks, or more equal values, than a short list).
+template <int EPL>
+__device__ __forceinline__ int pick_all(uint32_t (&k)[EPL], int K, int lane) {
+  int my_id = 0, bi = 0;
+  uint32_t best = 0u;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i)
     if (k[i] > best) {
       best = k[i];
       bi = i;
     }
-  }
-  my_id = 0;
-  float prev = INFINITY;
-  for (int kk = 0; kk < sh.K; ++kk) {
+  for (int kk = 0; kk < K; ++kk) {
     const uint32_t m = __reduce_max_sync(kFull, best);
     const int win = __ffs(__ballot_sync(kFull, best == m)) - 1;
     const int id = win * EPL + __shfl_sync(kFull, bi, win);
     if (lane == kk) my_id = id;
-    if (tol >= 0.f) {
-      const float v = unord32(m);
-      if (kk > 0 && !(prev - v > tol * (1.f + fabsf(v)))) sure = false;
-      prev = v;
-    }
     if (lane == win) {
       best = 0u;
       const int gone = bi;
@@ -148,11 +216,7 @@ __device__ __forceinline__ bool choose32(const float (&c)[EPL], float gscore, co
       }
     }
   }
-  if (tol >= 0.f) {  // the first value left out
-    const uint32_t m = __reduce_max_sync(kFull, best);
-    if (m != 0u && !(prev - unord32(m) > tol * (1.f + fabsf(prev)))) sure = false;
-  }
-  return sure;
+  return my_id;
 }
 
 // Largest of (v, i), the lower i among equals; i >= 0x7fffffff marks "none".
@@ -169,67 +233,54 @@ __device__ __forceinline__ void argmax64(double& v, int& i) {
   }
 }
 
-// The same choice in fp64, from the logits (rows whose fp32 values lie too close): by s + bias, or,
-// without a bias, by the logits, with only the groups ranked by sums of scores.
+// Exact choice value of a logit: s + bias.
+__device__ __forceinline__ double choice64(float x, bool sigmoid, float m, double inv_z, float bias) {
+  const double c = (x == kNegInf ? 0.0 : score64(x, sigmoid, m, inv_z)) + (double)bias;
+  return c == c ? c : (double)kNegInf;
+}
+
+// Open groups by exact scores (rows whose fp32 group scores lie too close).
 template <int EPL>
-__device__ __noinline__ int choose64(const float (&x)[EPL], const float* bias, bool sigmoid, const Shape& sh, int lane,
-                                     double* buf) {
-  float m = kNegInf;
-  double inv_z = 1.0;
-  if (!sigmoid) {
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) m = fmaxf(m, x[i]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-    double z = 0.0;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (x[i] > kNegInf) z += x[i] == m ? 1.0 : exp((double)x[i] - (double)m);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(kFull, z, o);
-    inv_z = z > 0.0 ? 1.0 / z : 0.0;
-  }
-  double c[EPL];
+__device__ __noinline__ unsigned open_groups64(const float (&x)[EPL], const float* bias, bool sigmoid, float m,
+                                               double inv_z, const Shape& sh, int lane, double* buf) {
+  double c[EPL], g1, g2;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     const int e = lane * EPL + i;
     c[i] = x[i];
-    if (bias != nullptr)
-      c[i] = e < sh.E ? (x[i] == kNegInf ? 0.0 : score64(x[i], sigmoid, m, inv_z)) + (double)bias[e] : (double)kNegInf;
-    if (!(c[i] == c[i])) c[i] = (double)kNegInf;
+    if (bias != nullptr) c[i] = e < sh.E ? choice64(x[i], sigmoid, m, inv_z, bias[e]) : (double)kNegInf;
   }
-  unsigned open = kFull;
-  if (sh.groups > 1) {
-    double g1, g2;
-    group_top2<EPL, double>(c, sh, lane, buf, g1, g2);
-    double g = g1;
-    if (sh.top2 && sh.gsize > 1) {
-      if (bias == nullptr) {
-        g1 = g1 == (double)kNegInf ? 0.0 : score64((float)g1, sigmoid, m, inv_z);
-        g2 = g2 == (double)kNegInf ? 0.0 : score64((float)g2, sigmoid, m, inv_z);
-      }
-      g = g1 + g2;
+  group_top2<EPL, double>(c, sh, lane, buf, g1, g2);
+  double g = g1;
+  if (sh.top2 && sh.gsize > 1) {
+    if (bias == nullptr) {
+      g1 = choice64((float)g1, sigmoid, m, inv_z, 0.f);
+      g2 = choice64((float)g2, sigmoid, m, inv_z, 0.f);
     }
-    bool taken = lane >= sh.groups;
-    open = 0;
-    for (int t = 0; t < sh.top_groups; ++t) {
-      double v = g;
-      int i = taken ? 0x7fffffff : lane;
-      argmax64(v, i);
-      open |= 1u << i;
-      if (lane == i) taken = true;
-    }
+    g = g1 + g2;
   }
-  unsigned live = 0;
+  bool taken = lane >= sh.groups;
+  unsigned open = 0;
+  for (int t = 0; t < sh.top_groups; ++t) {
+    double v = g;
+    int i = taken ? 0x7fffffff : lane;
+    argmax64(v, i);
+    open |= 1u << i;
+    if (lane == i) taken = true;
+  }
+  return open;
+}
+
+// The K best experts by exact choice values among those of `live` (bit i: expert lane * EPL + i).
+template <int EPL>
+__device__ __noinline__ int pick_all64(const float (&x)[EPL], const float* bias, bool sigmoid, float m, double inv_z,
+                                       unsigned live, int K, int lane) {
+  double c[EPL];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane * EPL + i;
-    bool in = e < sh.E;
-    if (sh.groups > 1 && in) in = (open >> (e / sh.gsize)) & 1u;
-    if (in) live |= 1u << i;
-  }
+  for (int i = 0; i < EPL; ++i)
+    c[i] = (live >> i) & 1u ? choice64(x[i], sigmoid, m, inv_z, bias[lane * EPL + i]) : 0.0;
   int my_id = 0;
-  for (int kk = 0; kk < sh.K; ++kk) {
+  for (int kk = 0; kk < K; ++kk) {
     double v = 0.0;
     int id = 0x7fffffff;
 #pragma unroll
@@ -246,9 +297,10 @@ __device__ __noinline__ int choose64(const float (&x)[EPL], const float* bias, b
 }
 
 template <int EPL, bool F32>
-__global__ void __launch_bounds__(kWarps * 32) route_scored_kernel(const RouteScoredParams p, const Shape sh, int vec) {
+__global__ void __launch_bounds__(kWarps * 32) route_scored_kernel(const RouteScoredParams p, const Shape sh, int vec, int vecb) {
   pdl_wait();
   pdl_trigger();
+  __shared__ uint2 cand[kWarps][32];
   extern __shared__ double dynbuf[];  // per warp E doubles (only when a group starts inside a lane)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x * kWarps + warp;
@@ -279,7 +331,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_scored_kernel(const RouteSc
   }
   const bool sigm = p.sigmoid;
   float m = 0.f, z = 1.f;
-  const bool need_z = !sigm && (p.bias != nullptr || !p.renorm);
+  const bool need_z = !sigm && !p.renorm;  // (the weights' denominator)
   if (!sigm) {
     m = kNegInf;
 #pragma unroll
@@ -294,46 +346,97 @@ __global__ void __launch_bounds__(kWarps * 32) route_scored_kernel(const RouteSc
       for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(kFull, z, o);
     }
   }
-  const float inv_z = z > 0.f ? 1.f / z : 0.f;
-  // Error of the fp32 choice values: a score (absolute value <= 1) is off by less than 4e-7 (fast
-  // exponential and divide), adding the bias rounds by 2^-24 of the sum; so 1e-6 (1 + |c|) covers a
-  // difference of two, and twice that a difference of two sums of two.
-  int my_id;
-  bool sure;
+  double inv_z64 = 1.0;  // exact softmax denominator: needed where scores meet a bias
+  if (!sigm && p.bias != nullptr) {
+    double z64 = 0.0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (x[i] > kNegInf) z64 += x[i] == m ? 1.0 : exp((double)x[i] - (double)m);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) z64 += __shfl_xor_sync(kFull, z64, o);
+    inv_z64 = z64 > 0.0 ? 1.0 / z64 : 0.0;
+  }
+  // fp32 choice values. A score (absolute value <= 1) is off by less than 4e-7 (argument rounded by
+  // 2^-24 of itself, exponential 2 ulp, reciprocal 1 ulp), adding the bias rounds by 2^-24 of the sum:
+  // 2e-6 (1 + |c|) is more than the error of a difference of two, or of two sums of two.
+  constexpr float kTol = 2e-6f;
+  float c[EPL];
   if (p.bias == nullptr) {
-    float g = 0.f, tol_g = -1.f;
-    if (sh.groups > 1) {
-      float g1, g2;
-      group_top2<EPL, float>(x, sh, lane, reinterpret_cast<float*>(buf), g1, g2);
-      g = g1;
-      if (sh.top2 && sh.gsize > 1) {
-        auto sc = [&](float v) {
-          if (v == kNegInf) return 0.f;
-          return sigm ? __fdividef(1.f, 1.f + __expf(-v)) : (v == m ? 1.f : __expf(v - m));
-        };
-        g = sc(g1) + sc(g2);
-        tol_g = 2e-6f;
-      }
-    }
-    sure = choose32<EPL>(x, g, sh, lane, tol_g, -1.f, my_id);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) c[i] = x[i];
   } else {
-    float c[EPL];
+    const float inv_z = (float)inv_z64;
+    float b[EPL];
+    if (EPL % 4 == 0 && vecb && (lane + 1) * EPL <= E) {
+#pragma unroll
+      for (int i = 0; i < EPL / 4; ++i) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p.bias + lane * EPL) + i);
+        b[4 * i] = v.x;
+        b[4 * i + 1] = v.y;
+        b[4 * i + 2] = v.z;
+        b[4 * i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) b[i] = lane * EPL + i < E ? __ldg(p.bias + lane * EPL + i) : kNegInf;
+    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      c[i] = clean((sigm ? sigmoid_fast(x[i]) : (x[i] == m ? 1.f : exp_fast(x[i] - m)) * inv_z) + b[i]);
+  }
+  unsigned open = kFull;
+  if (sh.groups > 1) {
+    float g1, g2, g, tol = -1.f;
+    group_top2<EPL, float>(c, sh, lane, reinterpret_cast<float*>(buf), g1, g2);
+    g = g1;
+    if (p.bias != nullptr) tol = kTol;
+    if (sh.top2 && sh.gsize > 1) {
+      if (p.bias == nullptr) {
+        g1 = g1 == kNegInf ? 0.f : sigm ? sigmoid_fast(g1) : (g1 == m ? 1.f : exp_fast(g1 - m));
+        g2 = g2 == kNegInf ? 0.f : sigm ? sigmoid_fast(g2) : (g2 == m ? 1.f : exp_fast(g2 - m));
+      }
+      g = g1 + g2;
+      tol = kTol;
+    }
+    bool sure;
+    open = open_groups32(g, sh, lane, tol, sure);
+    if (!sure) open = open_groups64<EPL>(x, p.bias, sigm, m, inv_z64, sh, lane, buf);
+  }
+  uint32_t k[EPL];
+  unsigned live = 0;
+  if (sh.lanes > 0) {  // the lane's experts are of one group
+    const bool in = (open >> (lane / sh.lanes)) & 1u;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      k[i] = in && lane * EPL + i < E ? ord32(c[i]) : 0u;
+      live |= (k[i] != 0u ? 1u : 0u) << i;
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
       const int e = lane * EPL + i;
-      float s = 0.f;
-      if (x[i] > kNegInf) s = sigm ? __fdividef(1.f, 1.f + __expf(-x[i])) : (x[i] == m ? 1.f : __expf(x[i] - m)) * inv_z;
-      c[i] = e < E ? clean(s + __ldg(p.bias + e)) : kNegInf;
+      k[i] = e < E && ((open >> (e / sh.gsize)) & 1u) ? ord32(c[i]) : 0u;
+      live |= (k[i] != 0u ? 1u : 0u) << i;
     }
-    float g = 0.f;
-    if (sh.groups > 1) {
-      float g1, g2;
-      group_top2<EPL, float>(c, sh, lane, reinterpret_cast<float*>(buf), g1, g2);
-      g = sh.top2 && sh.gsize > 1 ? g1 + g2 : g1;
-    }
-    sure = choose32<EPL>(c, g, sh, lane, 2e-6f, 1e-6f, my_id);
   }
-  if (!sure) my_id = choose64<EPL>(x, p.bias, sigm, sh, lane, buf);
+  int my_id, listed = 33;
+  uint2 my;
+  if (sh.K <= kListK) listed = short_list<EPL>(k, sh.K, p.bias == nullptr ? 0.f : kTol, lane, cand[warp], my);
+  if (p.bias == nullptr) {
+    my_id = listed <= 32 ? pick_list<false>(my.x, 0u, (int)my.y, sh.K, lane) : pick_all<EPL>(k, sh.K, lane);
+  } else if (listed <= 32) {
+    uint32_t hi = 0u, lo = 0u;
+    if (lane < listed) {
+      const float xv = clean(F32 ? lf[my.y] : __bfloat162float(lh[my.y]));
+      unsigned long long u = __double_as_longlong(choice64(xv, sigm, m, inv_z64, __ldg(p.bias + my.y)) + 0.0);
+      u ^= (unsigned long long)((long long)u >> 63) | 0x8000000000000000ull;
+      hi = (uint32_t)(u >> 32);
+      lo = (uint32_t)u;
+    }
+    my_id = pick_list<true>(hi, lo, (int)my.y, sh.K, lane);
+  } else {
+    my_id = pick_all64<EPL>(x, p.bias, sigm, m, inv_z64, live, sh.K, lane);
+  }
   // weights: lane k takes pick k, in fp32 with the accurate exponential and divide
   const bool on = lane < sh.K;
   const float xi = on ? clean(F32 ? lf[my_id] : __bfloat162float(lh[my_id])) : kNegInf;
@@ -364,11 +467,11 @@ __global__ void __launch_bounds__(kWarps * 32) route_scored_kernel(const RouteSc
 }
 
 template <int EPL>
-cudaError_t launch_epl(const RouteScoredParams& p, const Shape& sh, int vec, cudaStream_t s) {
+cudaError_t launch_epl(const RouteScoredParams& p, const Shape& sh, int vec, int vecb, cudaStream_t s) {
   const dim3 grid((p.T + kWarps - 1) / kWarps);
   const size_t smem = sh.lanes > 0 ? 0 : (size_t)kWarps * sh.E * sizeof(double);
-  if (p.f32) SQ_LAUNCH((route_scored_kernel<EPL, true>), grid, dim3(kWarps * 32), smem, s, 1, p, sh, vec);
-  else SQ_LAUNCH((route_scored_kernel<EPL, false>), grid, dim3(kWarps * 32), smem, s, 1, p, sh, vec);
+  if (p.f32) SQ_LAUNCH((route_scored_kernel<EPL, true>), grid, dim3(kWarps * 32), smem, s, 1, p, sh, vec, vecb);
+  else SQ_LAUNCH((route_scored_kernel<EPL, false>), grid, dim3(kWarps * 32), smem, s, 1, p, sh, vec, vecb);
   return cudaGetLastError();
 }
 
@@ -394,17 +497,18 @@ cudaError_t moe_route_scored_launch(const RouteScoredParams& p, cudaStream_t s) 
   for (int c : kEpl)
     if (!epl && c * 32 >= p.E) epl = c;
   const int vec = !p.f32 && p.ld % 8 == 0 && reinterpret_cast<uintptr_t>(p.logits) % 16 == 0;
+  const int vecb = p.bias != nullptr && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
   switch (epl) {
-    case 1: return launch_epl<1>(p, sh, vec, s);
-    case 2: return launch_epl<2>(p, sh, vec, s);
-    case 3: return launch_epl<3>(p, sh, vec, s);
-    case 4: return launch_epl<4>(p, sh, vec, s);
-    case 5: return launch_epl<5>(p, sh, vec, s);
-    case 6: return launch_epl<6>(p, sh, vec, s);
-    case 8: return launch_epl<8>(p, sh, vec, s);
-    case 10: return launch_epl<10>(p, sh, vec, s);
-    case 12: return launch_epl<12>(p, sh, vec, s);
-    default: return launch_epl<16>(p, sh, vec, s);
+    case 1: return launch_epl<1>(p, sh, vec, vecb, s);
+    case 2: return launch_epl<2>(p, sh, vec, vecb, s);
+    case 3: return launch_epl<3>(p, sh, vec, vecb, s);
+    case 4: return launch_epl<4>(p, sh, vec, vecb, s);
+    case 5: return launch_epl<5>(p, sh, vec, vecb, s);
+    case 6: return launch_epl<6>(p, sh, vec, vecb, s);
+    case 8: return launch_epl<8>(p, sh, vec, vecb, s);
+    case 10: return launch_epl<10>(p, sh, vec, vecb, s);
+    case 12: return launch_epl<12>(p, sh, vec, vecb, s);
+    default: return launch_epl<16>(p, sh, vec, vecb, s);
   }
 }
 
