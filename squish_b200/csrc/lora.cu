@@ -620,7 +620,7 @@ cudaError_t launch_lora(const LoraParams& p, int C, cudaStream_t s) {
   const size_t smem = small ? smem16 : (size_t)Tile64<R, SILU>::kSmem;
   auto* kern = small ? lora_row16_kernel<R, SILU> : lora_row64_kernel<R, SILU>;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_smem(kern, (int)smem);
     if (e != cudaSuccess) return e;
   }
   SQ_LAUNCH(kern, dim3(p.max_tiles, 1, C), dim3(kThreads), smem, s, C, p);
@@ -638,8 +638,7 @@ cudaError_t lora_plan_launch(const LoraPlanParams& p, cudaStream_t s) {
   if (p.slots < 1 || p.slots > kLoraMaxSlots || (p.tm != 16 && p.tm != 64)) return cudaErrorInvalidValue;
   const size_t smem = (size_t)(kPlanWarps * (p.slots + 1) + 2 * (p.slots + 2)) * sizeof(int);
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(lora_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (kPlanWarps * (kLoraMaxSlots + 1) + 2 * (kLoraMaxSlots + 2)) * 4);
+    const cudaError_t e = allow_smem(lora_plan_kernel, (kPlanWarps * (kLoraMaxSlots + 1) + 2 * (kLoraMaxSlots + 2)) * 4);
     if (e != cudaSuccess) return e;
   }
   SQ_LAUNCH(lora_plan_kernel, dim3(1), dim3(kPlanThreads), smem, s, 1, p);
@@ -651,7 +650,6 @@ cudaError_t lora_add_launch(const LoraParams& p, int num_sms, cudaStream_t s) {
   if (p.K % 8 || p.N % 8 || (p.silu && p.N % 128) || (p.tm != 16 && p.tm != 64)) return cudaErrorInvalidValue;
   int C = 8;
   while (C > 1 && p.max_tiles * C > 4 * num_sms) C >>= 1;
-  if (const char* e = getenv("LORA_C")) C = atoi(e);
   switch (p.R) {
     case 16: return launch_rank<16>(p, C, s);
     case 32: return launch_rank<32>(p, C, s);

@@ -836,7 +836,7 @@ template <int C>
 cudaError_t launch_c(const SampleUniformParams& p, cudaStream_t s) {
   // histogram, the row's counts of the CTA's share (C > 1), list of its non-empty bins
   constexpr size_t smem = (size_t)(kHist + (C > 1 ? 2 * kMagN / C + 4 : 0)) * sizeof(int) + (size_t)(2 * kMagN / C + 8) * 2;
-  cudaError_t e = cudaFuncSetAttribute(sample_uniform_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_smem(sample_uniform_kernel<C>, (int)smem);
   if (e != cudaSuccess) return e;
   SQ_LAUNCH(sample_uniform_kernel<C>, dim3(p.B, 1, C), dim3(kThreads), smem, s, C, p);
   return cudaGetLastError();

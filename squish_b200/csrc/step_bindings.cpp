@@ -50,9 +50,7 @@ constexpr auto BF16 = torch::kBFloat16;
 
 // ------------------------------------------------------------------ step layout
 void step_layout(torch::Tensor ctx, torch::Tensor q, torch::Tensor tables, torch::Tensor free_pages, int64_t page,
-                 int64_t tile, torch::Tensor q_start, torch::Tensor kv_len, torch::Tensor positions,
-                 torch::Tensor slots, torch::Tensor token_seq, torch::Tensor last_row, torch::Tensor tile_seq,
-                 torch::Tensor tile_q0, torch::Tensor totals, torch::Tensor status) {
+                 int64_t tile, torch::Tensor out, int64_t max_seqs, int64_t cap, int64_t tcap, torch::Tensor status) {
   const auto dev = cuda_device(ctx, "ctx_len");
   const int64_t B = ctx.numel();
   TORCH_CHECK(B >= 1 && B <= sq::kLayoutMaxSeqs, "a step has 1..", str(sq::kLayoutMaxSeqs), " sequences, not ", str(B));
@@ -70,23 +68,34 @@ void step_layout(torch::Tensor ctx, torch::Tensor q, torch::Tensor tables, torch
   p.bt_stride = (int)tables.stride(0);
   p.bt_width = (int)tables.size(1);
   p.free_pages = arr<int>(free_pages, "free_pages", I32, dev, 0);
-  const int64_t cap = positions.numel(), tcap = tile_seq.numel();
-  TORCH_CHECK(cap <= (1 << 30) && tcap <= (1 << 30) && free_pages.numel() <= (1 << 30), "buffers above 2^30 elements");
+  TORCH_CHECK(cap >= 0 && tcap >= 0 && cap <= (1 << 28) && tcap <= (1 << 28) && free_pages.numel() <= (1 << 30),
+              "step buffers above 2^28 rows");
+  TORCH_CHECK(B <= max_seqs, "a step of ", str(B), " sequences in a layout of ", str(max_seqs));
   p.n_free = (int)free_pages.numel();
   p.B = (int)B;
   p.page_size = (int)page;
   p.tile = (int)tile;
   p.token_cap = (int)cap;
   p.tile_cap = (int)tcap;
-  p.q_start = arr<int>(q_start, "q_start", I32, dev, B + 1);
-  p.kv_len = arr<int>(kv_len, "kv_len", I32, dev, B);
-  p.positions = arr<int>(positions, "positions", I32, dev, 0);
-  p.slots = arr<int>(slots, "slots", I32, dev, cap);
-  p.token_seq = arr<int>(token_seq, "token_seq", I32, dev, cap);
-  p.last_row = arr<int>(last_row, "last_row", I32, dev, B);
-  p.tile_seq = arr<int>(tile_seq, "tile_seq", I32, dev, 0);
-  p.tile_q0 = arr<int>(tile_q0, "tile_q0", I32, dev, tcap);
-  p.totals = arr<int>(totals, "totals", I32, dev, 3);
+  // one buffer, its rows in this order, each padded to a multiple of four (ops.step.StepLayout)
+  auto pad = [](int64_t n) { return (n + 3) / 4 * 4; };
+  int* at = arr<int>(out, "the step layout", I32, dev,
+                     pad(max_seqs + 1) + 2 * pad(max_seqs) + 4 + 3 * pad(cap) + 2 * pad(tcap));
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(at) % 16 == 0, "the step layout must be 16-byte aligned");
+  auto row = [&](int64_t n) {
+    int* r = at;
+    at += pad(n);
+    return r;
+  };
+  p.q_start = row(max_seqs + 1);
+  p.kv_len = row(max_seqs);
+  p.last_row = row(max_seqs);
+  p.totals = row(3);
+  p.positions = row(cap);
+  p.slots = row(cap);
+  p.token_seq = row(cap);
+  p.tile_seq = row(tcap);
+  p.tile_q0 = row(tcap);
   p.status = arr<int>(status, "status", I32, dev, 1);
   const c10::cuda::CUDAGuard g(dev);
   ok(sq::step_layout_launch(p, sms(), stream()), "step_layout");

@@ -8,6 +8,27 @@
 
 namespace sq {
 
+// Dynamic shared memory above 48 KB has to be allowed once per kernel and device (a driver call of its
+// own: not one per launch). Kernels without a size that varies call it with their largest.
+template <typename K>
+cudaError_t allow_smem(K* kernel, int bytes) {
+  struct Done {
+    const void* kernel;
+    int device;
+  };
+  static thread_local Done done[64];
+  static thread_local int n = 0;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const void* k = reinterpret_cast<const void*>(kernel);
+  for (int i = 0; i < n; ++i)
+    if (done[i].kernel == k && done[i].device == dev) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && n < 64) done[n++] = {k, dev};
+  return e;
+}
+
 // ---------------------------------------------------------------- step layout (step_layout.cu)
 constexpr int kLayoutMaxSeqs = 8192;       // per-sequence prefixes live in shared memory (16 B each)
 constexpr int kLayoutPadQ0 = 1 << 30;      // first query of a padding tile: past every chunk's end
@@ -21,7 +42,7 @@ struct StepLayoutParams {
   int B, page_size, tile, token_cap, tile_cap;
   int* q_start;    // [B + 1]
   int* kv_len;     // [B]
-  int* positions;  // [token_cap]
+  int* positions;  // [token_cap], like the next two 16-byte aligned and padded to a multiple of 4
   int* slots;      // [token_cap]
   int* token_seq;  // [token_cap]
   int* last_row;   // [B]

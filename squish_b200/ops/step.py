@@ -37,14 +37,16 @@ class StepLayout:
             raise ValueError("a step layout holds at least one sequence and one token")
         if max_tiles is None:
             max_tiles = max_tokens // tile + min(max_seqs, max_tokens)
-        self.max_seqs, self.tile = max_seqs, tile
-
-        def buf(n):
-            return torch.zeros(n, dtype=torch.int32, device=device)
-
-        self._q_start, self._kv_len, self._last_row = buf(max_seqs + 1), buf(max_seqs), buf(max_seqs)
-        self.positions, self.slots, self.token_seq = buf(max_tokens), buf(max_tokens), buf(max_tokens)
-        self.tile_seq, self.tile_q0, self.totals = buf(max_tiles), buf(max_tiles), buf(3)
+        self.max_seqs, self.max_tokens, self.max_tiles, self.tile = max_seqs, max_tokens, max_tiles, tile
+        # one buffer (one argument of the launch), each row padded to a multiple of four
+        sizes = (max_seqs + 1, max_seqs, max_seqs, 3, max_tokens, max_tokens, max_tokens, max_tiles, max_tiles)
+        self.buf = torch.zeros(sum((n + 3) // 4 * 4 for n in sizes), dtype=torch.int32, device=device)
+        rows, at = [], 0
+        for n in sizes:
+            rows.append(self.buf[at:at + n])
+            at += (n + 3) // 4 * 4
+        (self._q_start, self._kv_len, self._last_row, self.totals, self.positions, self.slots, self.token_seq,
+         self.tile_seq, self.tile_q0) = rows
         self._narrow(max_seqs)
 
     def _narrow(self, b: int) -> None:
@@ -70,9 +72,8 @@ def step_layout(ctx_len: torch.Tensor, q_len: torch.Tensor, block_tables: torch.
     if b != out.seqs:
         out._narrow(b)
     ws = ws or workspace(ctx_len.device)
-    native().step_layout(ctx_len, q_len, block_tables, free_pages, page_size, out.tile, out.q_start, out.kv_len,
-                         out.positions, out.slots, out.token_seq, out.last_row, out.tile_seq, out.tile_q0, out.totals,
-                         ws.status)
+    native().step_layout(ctx_len, q_len, block_tables, free_pages, page_size, out.tile, out.buf, out.max_seqs,
+                         out.max_tokens, out.max_tiles, ws.status)
     _count()
     return out
 

@@ -18,7 +18,7 @@ def test_cpu_tensors_are_refused():
     f = torch.zeros(2)
     C = native()
     with pytest.raises(RuntimeError, match="ctx_len must be a CUDA tensor"):
-        C.step_layout(i32(2), i32(2), i32(2, 4), i32(8), 16, 32, *[i32(8)] * 10)
+        C.step_layout(i32(2), i32(2), i32(2, 4), i32(8), 16, 32, i32(64), 2, 4, 4, i32(1))
     with pytest.raises(RuntimeError, match="logits must be a CUDA tensor"):
         ops.sample_uniform(x, f, i32(2))
     with pytest.raises(RuntimeError, match="logits must be a CUDA tensor"):

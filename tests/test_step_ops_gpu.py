@@ -71,7 +71,7 @@ def test_layout_small(cuda, ctx, q, ps):
     run_layout(cuda, ctx, q, ps)
 
 
-@pytest.mark.parametrize("B,maxq,maxc,ps", [(64, 1, 2000, 16), (257, 40, 300, 16), (1000, 3, 5000, 32), (8192, 2, 40, 8),
+@pytest.mark.parametrize("B,maxq,maxc,ps", [(64, 1, 2000, 16), (257, 40, 300, 16), (400, 800, 90, 16), (1000, 3, 5000, 32), (8192, 2, 40, 8),
                                             (300, 700, 90, 24)])
 def test_layout_random(cuda, B, maxq, maxc, ps):
     rng = random.Random(B)
