@@ -20,6 +20,8 @@
 // 2^-9 |h| per rank to every column. The rank is small, so the second product costs no time.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "kernels.h"
 #include "launch.cuh"
 #include "sm100.cuh"
@@ -380,7 +382,7 @@ __global__ void __launch_bounds__(kThreads) lora_row16_kernel(const LoraParams p
   if (rank > 0) cl.sync();  // peers may still read this CTA's share
 }
 
-// ---------------------------------------------------------------- tiles of 64 rows (prefill)
+// ---------------------------------------------------------------- tiles of 128 rows (prefill)
 __device__ __forceinline__ void cp16(void* dst, const void* src, bool on) {  // 16 bytes, or zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
@@ -389,253 +391,428 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// Offset of 16-byte chunk c (0..7) of row r in a tile of 128-byte rows. A fragment load reads four
-// chunks of two neighbouring rows per phase: odd rows swap their halves, so they meet no bank twice.
-__device__ __forceinline__ int sw(int r, int c) { return r * 128 + ((c ^ ((r & 1) << 2)) << 4); }
+// Offset of 16-byte chunk c (0..7) of row r in a tile of 128-byte rows, 128-byte swizzle (the tensor
+// cores' operand layout; a row-per-lane read meets no bank twice either).
+__device__ __forceinline__ int sw(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+__device__ __forceinline__ uint8_t* align1k(uint8_t* p) {
+  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
+}
 
-// 8 warps: 4 row groups of 16 x 2 halves (of the rank tiles in the shrink, of the columns in the
-// expand). One ring of stages runs through both products: x and A in 64-wide steps of K, then y and
-// B in units of 64 columns (gate and up: 128), so the first units of y are in flight while the
-// cluster exchanges h. The loads are what bounds it: without the ring each warp waited for its own
-// fragments (8185 rows, K 4096, N 6144, rank 64: 240 us, 1.1 TB/s).
-template <int R, bool SILU>
-struct Tile64 {
-  static constexpr int G = SILU ? 2 : 1;
-  static constexpr int kStage = G * 64 * 128 + G * 64 * R * 2 > 64 * 128 + R * 128 ? G * 64 * 128 + G * 64 * R * 2
-                                                                                  : 64 * 128 + R * 128;
-  static constexpr int kPart = 64 * (R + 4) * 4, kH = 2 * 64 * (R + 8) * 2;
-  // as many stages as two resident CTAs leave room for, at least two
-  static constexpr int kFit = (113 * 1024 - kPart - kH - 1024) / kStage;
-  static constexpr int S = kFit > 5 ? 5 : kFit < 2 ? 2 : kFit;
-  static constexpr int kSmem = S * kStage + kPart + kH;
+// Two launches. The shrink: a cluster per tile, K split over its CTAs; x and A_s stream through a ring of
+// 64-wide steps into tcgen05 products that accumulate [128, R] in tensor memory, and the cluster's
+// shares leave h in a scratch buffer as two bf16 parts. The expand: a tile's h stays in shared memory
+// as the A operand (both parts, against the same B), y and B_s stream through a ring of 64-column units
+// (gate and up: 64 of each), and the epilogue adds the product in place of y, from where whole
+// 128-byte rows go out. The rows are gathered, so the ring is filled by cp.async, 16 bytes a thread.
+//
+// It is bound by bytes, so what it takes is few instructions per byte and enough of them in flight.
+// With mma.sync fragments (a warp 16 rows x 32 columns) the same ring was bound by instruction issue:
+// 8185 rows, K 4096, N 6144, rank 64: 72 us, against 240 us without a ring.
+template <int R>
+struct Shrink128 {
+  static constexpr int kStage = 128 * 128 + R * 128;
+  static constexpr int kPart = 128 * (R + 4) * 4;  // (in the ring, once it is empty)
+  static constexpr int kFit = (111 * 1024) / kStage;  // two CTAs per SM
+  static constexpr int S = kFit > 5 ? 5 : kFit;
+  static constexpr int kSmem = (S * kStage > kPart ? S * kStage : kPart) + 1024;
+  static constexpr int kCols = R < 32 ? 32 : R;
 };
 
-template <int R, bool SILU>
-__global__ void __launch_bounds__(kThreads) lora_row64_kernel(const LoraParams p) {
-  using TC = Tile64<R, SILU>;
-  constexpr int S = TC::S, G = TC::G;
-  constexpr int RH = R / 16;        // 8-wide rank tiles of a warp: 2 i + half
-  constexpr int PS = R + 4, HS = R + 8;
+template <int R>
+__global__ void __launch_bounds__(kThreads, 2) lora_shrink128_kernel(const LoraParams p) {
+  using TC = Shrink128<R>;
+  constexpr int S = TC::S, PS = R + 4;
+  static_assert(S >= 3 && TC::kStage % 1024 == 0, "ring");
   pdl_wait();
   pdl_trigger();
   if ((int)blockIdx.x >= *p.num_tiles) return;  // the whole cluster
   const int4 tile = p.tiles[blockIdx.x];
   const int slot = tile.x, cnt = tile.z;
   const int rank = slot >= 0 ? p.rank[slot] : 0;
-  if (rank <= 0 && p.in_place) return;
-  extern __shared__ __align__(128) uint8_t smem[];
-  float* part = reinterpret_cast<float*>(smem + S * TC::kStage);                         // [64][PS]
-  __nv_bfloat16* hh = reinterpret_cast<__nv_bfloat16*>(smem + S * TC::kStage + TC::kPart);  // [2][64][HS]
-  __shared__ int rows[64];
+  if (rank <= 0) return;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1k(smem_raw);
+  float* part = reinterpret_cast<float*>(smem);  // [128][PS]
+  __shared__ int rows[128];
+  __shared__ __align__(8) uint64_t done[S];
+  __shared__ uint32_t tmem_slot;
   cg::cluster_group cl = cg::this_cluster();
   const int C = gridDim.z, cr = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g = lane >> 2, t = lane & 3;
-  const int rw = warp >> 1, hf = warp & 1;
-  if (tid < 64) rows[tid] = tid < cnt ? p.order[tile.y + tid] : -1;
+  if (tid < 128) rows[tid] = tid < cnt ? p.order[tile.y + tid] : -1;
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(&done[i], 1);
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&tmem_slot, TC::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
   __syncthreads();
-  const int live = min(R, (rank + 15) / 16 * 16);
-  const int steps = rank > 0 ? (p.K + 63) / 64 : 0;
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int live = min(R, (rank + 15) / 16 * 16);  // ranks computed
+  const int steps = (p.K + 63) / 64;
   const int k0 = (int)((long long)steps * cr / C), n1 = (int)((long long)steps * (cr + 1) / C) - k0;
-  const int units = (p.N + 64 * G - 1) / (64 * G);
-  const int u0 = (int)((long long)units * cr / C), n2 = (int)((long long)units * (cr + 1) / C) - u0;
-  const __nv_bfloat16* as = p.a + (size_t)(slot < 0 ? 0 : slot) * R * p.K;
-  const __nv_bfloat16* bs = p.b + (size_t)(slot < 0 ? 0 : slot) * p.N * R;
 
-  // a thread copies chunk tid % 8 of rows tid / 8 and tid / 8 + 32 of a 64-row tile
+  // a thread copies chunk tid % 8 of rows tid / 8 + 32 j; the pointers run along
   const int lr = tid >> 3, lc = tid & 7;
-  const int ra = rows[lr], rb = rows[lr + 32];
-  const __nv_bfloat16* xa = p.x + (ra < 0 ? 0 : ra) * p.ldx + lc * 8;
-  const __nv_bfloat16* xb = p.x + (rb < 0 ? 0 : rb) * p.ldx + lc * 8;
-  const __nv_bfloat16* ya = p.y + (ra < 0 ? 0 : ra) * p.ldy + lc * 8;
-  const __nv_bfloat16* yb = p.y + (rb < 0 ? 0 : rb) * p.ldy + lc * 8;
-  int wr = 0, rd = 0;  // offsets of the next stage to fill and to use
-  auto next = [](int& at) { at = at == (S - 1) * TC::kStage ? 0 : at + TC::kStage; };
+  const __nv_bfloat16* px[4];
+  unsigned on = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = rows[lr + 32 * j];
+    on |= (r >= 0 ? 1u : 0u) << j;
+    px[j] = p.x + (r < 0 ? 0 : r) * p.ldx + k0 * 64 + lc * 8;
+  }
+  const __nv_bfloat16* pa = p.a + ((size_t)slot * R + lr) * p.K + k0 * 64 + lc * 8;
+  const size_t a32 = (size_t)32 * p.K;
+  const int so = sw(lr, lc);  // (rows + 32: the same swizzle)
+  int kk = k0 * 64 + lc * 8, wr = 0;  // this thread's k; next stage to fill
   auto issue = [&](int i) {
-    uint8_t* st = smem + wr;
-    next(wr);
+    uint8_t* st = smem + wr * TC::kStage;
+    wr = wr == S - 1 ? 0 : wr + 1;
     if (i < n1) {
-      const int k = (k0 + i) * 64;
-      const bool in = k + lc * 8 < p.K;
-      cp16(st + sw(lr, lc), in ? xa + k : p.x, in && ra >= 0);
-      cp16(st + sw(lr + 32, lc), in ? xb + k : p.x, in && rb >= 0);
-      uint8_t* sa = st + 64 * 128;
+      const bool in = kk < p.K;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        cp16(st + so + j * 4096, in ? px[j] : p.x, in && ((on >> j) & 1u));
+        px[j] += 64;
+      }
 #pragma unroll
       for (int r = 0; r < R; r += 32)
-        if (r + lr < live) cp16(sa + sw(r + lr, lc), in ? as + (size_t)(r + lr) * p.K + k + lc * 8 : as, in);
-    } else if (i < n1 + n2) {
-      const int col = (u0 + i - n1) * 64 * G;
-#pragma unroll
-      for (int q = 0; q < G; ++q) {
-        const int c = col + q * 64;
-        const bool in = c + lc * 8 < p.N;
-        cp16(st + q * 8192 + sw(lr, lc), in ? ya + c : p.y, in && ra >= 0);
-        cp16(st + q * 8192 + sw(lr + 32, lc), in ? yb + c : p.y, in && rb >= 0);
-      }
-      uint8_t* sb = st + G * 8192;
-      constexpr int CH = R / 8;  // 16-byte pieces of a B row
-      const int c = tid % CH;
-      if (c * 8 < live) {
-#pragma unroll
-        for (int n = tid / CH; n < G * 64; n += kThreads / CH) {
-          const bool in = col + n < p.N;
-          const __nv_bfloat16* src = in ? bs + (size_t)(col + n) * R + c * 8 : bs;
-          if (R >= 64) cp16(sb + (c >> 3) * (G * 64 * 128) + sw(n, c & 7), src, in);
-          else cp16(sb + n * R * 2 + c * 16, src, in);
-        }
-      }
+        if (r + lr < live) cp16(st + 16384 + so + r * 128, in ? pa + (r / 32) * a32 : p.a, in);
+      pa += 64;
+      kk += 64;
     }
     cp_commit();
   };
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) issue(i);
-
-  // ---- shrink
-  if (rank > 0) {
-    float acc[RH][4];
-#pragma unroll
-    for (int i = 0; i < RH; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-    for (int i = 0; i < n1; ++i) {
-      cp_wait<S - 2>();
-      __syncthreads();
-      issue(i + S - 1);
-      const uint8_t* st = smem + rd;
-      next(rd);
-      const uint8_t* sa = st + 64 * 128;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 v0 = *reinterpret_cast<const uint4*>(st + sw(rw * 16 + g, h * 4 + t));
-        const uint4 v1 = *reinterpret_cast<const uint4*>(st + sw(rw * 16 + g + 8, h * 4 + t));
-        uint4 w[RH];
-#pragma unroll
-        for (int j = 0; j < RH; ++j)
-          if ((2 * j + hf) * 8 < live) w[j] = *reinterpret_cast<const uint4*>(sa + sw((2 * j + hf) * 8 + g, h * 4 + t));
-#pragma unroll
-        for (int j = 0; j < RH; ++j)
-          if ((2 * j + hf) * 8 < live) mma16816(acc[j], v0.x, v1.x, v0.y, v1.y, w[j].x, w[j].y);
-#pragma unroll
-        for (int j = 0; j < RH; ++j)
-          if ((2 * j + hf) * 8 < live) mma16816(acc[j], v0.z, v1.z, v0.w, v1.w, w[j].z, w[j].w);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < RH; ++j) {
-      const int c = (2 * j + hf) * 8 + 2 * t;
-      if ((2 * j + hf) * 8 >= live) break;
-      *reinterpret_cast<float2*>(part + (rw * 16 + g) * PS + c) = make_float2(acc[j][0], acc[j][1]);
-      *reinterpret_cast<float2*>(part + (rw * 16 + g + 8) * PS + c) = make_float2(acc[j][2], acc[j][3]);
-    }
-    cl.sync();
-    const float sc = p.scale[slot];
-    const int nv = live / 4;
-    for (int i = tid; i < 64 * nv; i += kThreads) {
-      const int r = i / nv, c = (i - r * nv) * 4;
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int q = 0; q < C; ++q) {
-        const float4 v = *reinterpret_cast<const float4*>(cl.map_shared_rank(part, q) + r * PS + c);
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
-      }
-      s.x *= sc;
-      s.y *= sc;
-      s.z *= sc;
-      s.w *= sc;
-      const uint32_t h01 = pack_bf16(s.x, s.y), h23 = pack_bf16(s.z, s.w);
-      *reinterpret_cast<uint2*>(hh + r * HS + c) = make_uint2(h01, h23);
-      *reinterpret_cast<uint2*>(hh + (64 + r) * HS + c) =
-          make_uint2(pack_bf16(s.x - lo_f(h01), s.y - hi_f(h01)), pack_bf16(s.z - lo_f(h23), s.w - hi_f(h23)));
-    }
-    __syncthreads();
-  }
-
-  // ---- expand
-  constexpr int KS = R == 16 ? 1 : R / 32;
-  uint4 fa[2][KS][2];
-#pragma unroll
-  for (int q = 0; q < 2; ++q)
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const __nv_bfloat16* src = hh + (q * 64 + rw * 16 + g + 8 * r) * HS;
-        fa[q][ks][r] = make_uint4(0, 0, 0, 0);
-        if (R == 16) {
-          if (rank > 0) {
-            const uint2 v = *reinterpret_cast<const uint2*>(src + t * 4);
-            fa[q][ks][r].x = v.x;
-            fa[q][ks][r].y = v.y;
-          }
-        } else if (ks * 32 + t * 8 < live) {
-          fa[q][ks][r] = *reinterpret_cast<const uint4*>(src + ks * 32 + t * 8);
-        }
-      }
-  const int row0 = rows[rw * 16 + g], row1 = rows[rw * 16 + g + 8];
-  for (int i = n1; i < n1 + n2; ++i) {
+  const uint32_t idesc = idesc_bf16_f32(128, live);
+  int rd = 0;
+  for (int i = 0; i < n1; ++i) {
     cp_wait<S - 2>();
+    fence_proxy_async_smem();
     __syncthreads();
-    issue(i + S - 1);
-    const uint8_t* st = smem + rd;
-    next(rd);
-    const uint8_t* sb = st + G * 8192;
-    float acc[G][4][4];
+    if (warp == 0) {
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t a = smem_u32(smem + rd * TC::kStage), b = a + 16384;
 #pragma unroll
-    for (int q = 0; q < G; ++q) {
-      start_from(acc[q], *reinterpret_cast<const uint4*>(st + q * 8192 + sw(rw * 16 + g, hf * 4 + t)),
-                 *reinterpret_cast<const uint4*>(st + q * 8192 + sw(rw * 16 + g + 8, hf * 4 + t)));
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        if (ks * 32 >= live) break;
-        uint4 w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int n = q * 64 + hf * 32 + (g >> 1) * 8 + 2 * j + (g & 1);
-          w[j] = make_uint4(0, 0, 0, 0);
-          if (R == 16) {
-            const uint2 v = *reinterpret_cast<const uint2*>(sb + n * R * 2 + t * 8);
-            w[j].x = v.x;
-            w[j].y = v.y;
-          } else if (ks * 32 + t * 8 < live) {
-            if (R >= 64) w[j] = *reinterpret_cast<const uint4*>(sb + (ks >> 1) * (G * 64 * 128) + sw(n, (ks & 1) * 4 + t));
-            else w[j] = *reinterpret_cast<const uint4*>(sb + n * R * 2 + t * 16);
-          }
-        }
-        expand_step<R>(acc[q], fa[1][ks], fa[0][ks], w);
+        for (int k = 0; k < 4; ++k)
+          mma_bf16_ss(tmem, sdesc_sw128(a + k * 32), sdesc_sw128(b + k * 32), idesc, (i > 0 || k > 0) ? 1u : 0u);
+        mma_commit(&done[rd]);
       }
+      __syncwarp();
     }
-    const int oc = (u0 + i - n1) * 64 + hf * 32 + t * 8;
-    if (SILU || oc < p.N) {
-      if (row0 >= 0) *reinterpret_cast<uint4*>(p.out + row0 * p.ldo + oc) = finish<SILU, G>(acc, 0);
-      if (row1 >= 0) *reinterpret_cast<uint4*>(p.out + row1 * p.ldo + oc) = finish<SILU, G>(acc, 1);
-    }
+    // the stage to fill next is the one that the step before this one read
+    if (i > 0) mbar_wait(&done[rd == 0 ? S - 1 : rd - 1], (uint32_t)((i - 1) / S) & 1u, p.status, SQ_ERR_TIMEOUT_ACC);
+    issue(i + S - 1);
+    rd = rd == S - 1 ? 0 : rd + 1;
   }
-  if (rank > 0) cl.sync();  // peers may still read this CTA's share
+  if (n1 > 0) mbar_wait(&done[(n1 - 1) % S], (uint32_t)((n1 - 1) / S) & 1u, p.status, SQ_ERR_TIMEOUT_ACC);
+  cp_wait<0>();
+  __syncthreads();  // the ring is empty: its memory takes the shares
+  tc_fence_after();
+  {
+    const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * (R / 2);
+    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c0;
+    float* dst = part + row * PS + c0;
+#pragma unroll
+    for (int c = 0; c < R / 2; c += 8) {
+      uint32_t v[8];
+      tmem_ld8(at + c, v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int q = 0; q < 8; q += 4)
+        *reinterpret_cast<float4*>(dst + c + q) =
+            n1 > 0 ? make_float4(__uint_as_float(v[q]), __uint_as_float(v[q + 1]), __uint_as_float(v[q + 2]),
+                                 __uint_as_float(v[q + 3]))
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    tc_fence_before();
+  }
+  cl.sync();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TC::kCols);
+  }
+  // h of this CTA's share of the rows: the sum of the CTAs' shares of K, in rank order, scaled
+  const float sc = p.scale[slot];
+  const int r0 = 128 * cr / C, r1 = min(cnt, 128 * (cr + 1) / C);
+  const int nv = live / 4;
+  for (int i = tid; i < (r1 - r0) * nv; i += kThreads) {
+    const int q0 = i / nv, r = r0 + q0, c = (i - q0 * nv) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < C; ++q) {
+      const float4 v = *reinterpret_cast<const float4*>(cl.map_shared_rank(part, q) + r * PS + c);
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
+    s.x *= sc;
+    s.y *= sc;
+    s.z *= sc;
+    s.w *= sc;
+    const uint32_t h01 = pack_bf16(s.x, s.y), h23 = pack_bf16(s.z, s.w);
+    __nv_bfloat16* h = p.h + (size_t)(tile.y + r) * 2 * R + c;
+    *reinterpret_cast<uint2*>(h) = make_uint2(h01, h23);
+    *reinterpret_cast<uint2*>(h + R) =
+        make_uint2(pack_bf16(s.x - lo_f(h01), s.y - hi_f(h01)), pack_bf16(s.z - lo_f(h23), s.w - hi_f(h23)));
+  }
+  cl.sync();  // peers may still read this CTA's share
 }
 
 template <int R, bool SILU>
-cudaError_t launch_lora(const LoraParams& p, int C, cudaStream_t s) {
-  const bool small = p.tm == 16;
-  constexpr size_t smem16 = (size_t)kWarps * 16 * (R + 4) * 4 + (size_t)2 * 16 * (R + 8) * 2;
-  const size_t smem = small ? smem16 : (size_t)Tile64<R, SILU>::kSmem;
-  auto* kern = small ? lora_row16_kernel<R, SILU> : lora_row64_kernel<R, SILU>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = allow_smem(kern, (int)smem);
-    if (e != cudaSuccess) return e;
+struct Expand128 {
+  static constexpr int G = SILU ? 2 : 1;
+  // h: [128 rows][upper | lower] in 128-byte rows; B: [64 G columns][ranks] likewise, but up to rank 32
+  // gate and up share a row (64 bytes each)
+  static constexpr int kA = 128 * 128 * (R >= 64 ? R / 32 : 1);
+  static constexpr bool kPair = SILU && R <= 32;
+  static constexpr int kBRows = kPair ? 64 : 64 * G;
+  static constexpr int kB = kBRows * 128 * (R >= 64 ? R / 64 : 1);
+  static constexpr int kStage = G * 128 * 128 + kB;
+  static constexpr int kCtas = kA + 2 * kStage <= 111 * 1024 ? 2 : 1;  // per SM
+  static constexpr int kFit = ((kCtas == 2 ? 111 : 224) * 1024 - kA) / kStage;
+  static constexpr int S = kFit > 4 ? 4 : kFit;
+  static constexpr int kSmem = kA + S * kStage + 1024;
+  static constexpr int kCols = G * 64;
+};
+
+template <int R, bool SILU>
+__global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expand128_kernel(const LoraParams p) {
+  using TC = Expand128<R, SILU>;
+  constexpr int S = TC::S, G = TC::G;
+  static_assert(S >= 2 && TC::kStage % 1024 == 0, "ring");
+  // The launch before this one is the shrink, which lets this one start once everything before it is
+  // complete: the plan, y and B may be read at once, h after the wait.
+  const int4 tile = (int)blockIdx.y < *p.num_tiles ? p.tiles[blockIdx.y] : make_int4(-1, 0, 0, 0);
+  const int slot = tile.x, cnt = tile.z;
+  const int rank = slot >= 0 ? p.rank[slot] : 0;
+  if (cnt <= 0 || (rank <= 0 && p.in_place)) {
+    pdl_wait();
+    pdl_trigger();
+    return;
   }
-  SQ_LAUNCH(kern, dim3(p.max_tiles, 1, C), dim3(kThreads), smem, s, C, p);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ha = align1k(smem_raw);
+  uint8_t* ring = ha + TC::kA;
+  __shared__ int rows[128];
+  __shared__ __align__(8) uint64_t done;
+  __shared__ uint32_t tmem_slot;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid < 128) rows[tid] = tid < cnt ? p.order[tile.y + tid] : -1;
+  if (tid == 0) {
+    mbar_init(&done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&tmem_slot, TC::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int live = rank <= 0 ? 0 : min(R, (rank + 15) / 16 * 16);
+  const int units = (p.N + 64 * G - 1) / (64 * G);
+  const int u0 = blockIdx.x * p.units, n2 = min(p.units, units - u0);
+
+  // a thread copies chunk tid % 8 of rows tid / 8 + 32 j of y (and of out), and pieces of B rows
+  const int lr = tid >> 3, lc = tid & 7;
+  const __nv_bfloat16* py[4];
+  __nv_bfloat16* po[4];
+  unsigned on = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = rows[lr + 32 * j];
+    on |= (r >= 0 ? 1u : 0u) << j;
+    py[j] = p.y + (r < 0 ? 0 : r) * p.ldy + (long long)u0 * 64 * G + lc * 8;
+    po[j] = p.out + (r < 0 ? 0 : r) * p.ldo + (long long)u0 * 64 + lc * 8;
+  }
+  constexpr int CH = R / 8;          // 16-byte pieces of a B row
+  constexpr int BN = kThreads / CH;  // B rows per pass
+  const int bn = tid / CH, bc = tid % CH;
+  const __nv_bfloat16* pb = p.b + ((size_t)(slot < 0 ? 0 : slot) * p.N + (size_t)u0 * 64 * G + bn) * R + bc * 8;
+  const int so = sw(lr, lc);
+  int col = u0 * 64 * G, wr = 0;  // the unit's first column; next stage to fill
+  auto issue = [&](int i) {
+    uint8_t* st = ring + wr * TC::kStage;
+    wr = wr == S - 1 ? 0 : wr + 1;
+    if (i < n2) {
+      const bool in = SILU || col + lc * 8 < p.N;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int q = 0; q < G; ++q)
+          cp16(st + q * 16384 + so + j * 4096, in ? py[j] + q * 64 : p.y, in && ((on >> j) & 1u));
+        py[j] += 64 * G;
+      }
+      if (bc * 8 < live) {
+#pragma unroll
+        for (int k = 0; k < G * 64; k += BN) {
+          const int n = bn + k;
+          if (BN > G * 64 && n >= G * 64) break;
+          const bool ok = SILU || col + n < p.N;
+          const int at = TC::kPair ? sw(n & 63, (n >> 6) * 4 + bc) : (bc >> 3) * (G * 8192) + sw(n, bc & 7);
+          cp16(st + G * 16384 + at, ok ? pb + (size_t)k * R : p.b, ok);
+        }
+      }
+      pb += (size_t)64 * G * R;
+      col += 64 * G;
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) issue(i);
+  pdl_wait();
+  pdl_trigger();
+  if (live > 0) {  // h of the tile, as the A operand
+    for (int e = tid; e < 128 * 2 * CH; e += kThreads) {
+      const int r = e / (2 * CH), q = e / CH % 2, c = e % CH;
+      if (c * 8 < live) {
+        const int at = R >= 64 ? (q * (R / 64) + (c >> 3)) * 16384 + sw(r, c & 7) : sw(r, q * CH + c);
+        cp16(ha + at, r < cnt ? p.h + ((size_t)(tile.y + r) * 2 + q) * R + c * 8 : p.h, r < cnt);
+      }
+    }
+  }
+  cp_commit();
+  const int row = (warp & 3) * 32 + lane, hf = warp >> 2;  // this thread's row and half of the columns
+  const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  constexpr uint32_t idesc = idesc_bf16_f32(128, TC::kPair ? 64 : 64 * G);
+  int rd = 0;
+  for (int i = 0; i < n2; ++i) {
+    if (i == 0) cp_wait<0>();
+    else cp_wait<S - 2>();
+    fence_proxy_async_smem();
+    __syncthreads();
+    uint8_t* st = ring + rd * TC::kStage;
+    rd = rd == S - 1 ? 0 : rd + 1;
+    if (live > 0 && warp == 0) {
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t a = smem_u32(ha), b = smem_u32(st + G * 16384);
+#pragma unroll
+        for (int g = 0; g < (TC::kPair ? 2 : 1); ++g)  // (gate, up)
+#pragma unroll
+          for (int q = 1; q >= 0; --q)  // lower part first
+            for (int ks = 0; ks < live / 16; ++ks) {
+              const uint32_t ao = R >= 64 ? (q * (R / 64) + (ks >> 2)) * 16384 + (ks & 3) * 32 : (q * R / 16 + ks) * 32;
+              const uint32_t bo = TC::kPair ? g * 64 + ks * 32 : (ks >> 2) * (G * 8192) + (ks & 3) * 32;
+              mma_bf16_ss(tmem + g * 64, sdesc_sw128(a + ao), sdesc_sw128(b + bo), idesc, q == 0 || ks > 0 ? 1u : 0u);
+            }
+        mma_commit(&done);
+      }
+      __syncwarp();
+    }
+    issue(i + S - 1);  // (its stage was emptied by the step before this one)
+    if (live > 0) {
+      mbar_wait(&done, (uint32_t)i & 1u, p.status, SQ_ERR_TIMEOUT_ACC);
+      tc_fence_after();
+    }
+    // 32 output columns of the thread's row, 16 at a time, in place of y
+#pragma unroll
+    for (int c = 0; c < 32; c += 16) {
+      const int c0 = hf * 32 + c;
+      uint32_t v[G][16];
+      if (live > 0) {
+#pragma unroll
+        for (int q = 0; q < G; ++q) tmem_ld16(lanes + q * 64 + c0, v[q]);
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int q = 0; q < G; ++q)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[q][k] = 0u;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4* at = reinterpret_cast<uint4*>(st + sw(row, c0 / 8 + h));
+        const uint4 y = *at;
+        const uint32_t yw[4] = {y.x, y.y, y.z, y.w};
+        uint32_t uw[4] = {0, 0, 0, 0};
+        if (SILU) {
+          const uint4 x = *reinterpret_cast<const uint4*>(st + 16384 + sw(row, c0 / 8 + h));
+          uw[0] = x.x;
+          uw[1] = x.y;
+          uw[2] = x.z;
+          uw[3] = x.w;
+        }
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float f0 = lo_f(yw[k]) + __uint_as_float(v[0][8 * h + 2 * k]);
+          float f1 = hi_f(yw[k]) + __uint_as_float(v[0][8 * h + 2 * k + 1]);
+          if (SILU) {
+            f0 = silu_mul(f0, lo_f(uw[k]) + __uint_as_float(v[G - 1][8 * h + 2 * k]));
+            f1 = silu_mul(f1, hi_f(uw[k]) + __uint_as_float(v[G - 1][8 * h + 2 * k + 1]));
+          }
+          o[k] = pack_bf16(f0, f1);
+        }
+        *at = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (SILU || (u0 + i) * 64 + lc * 8 < p.N) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((on >> j) & 1u) *reinterpret_cast<uint4*>(po[j]) = *reinterpret_cast<const uint4*>(st + so + j * 4096);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) po[j] += 64;
+  }
+  cp_wait<0>();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TC::kCols);
+  }
+}
+
+template <int R, bool SILU>
+cudaError_t launch_lora(const LoraParams& p, int C, int num_sms, cudaStream_t s) {
+  if (p.tm == 16) {
+    constexpr size_t smem = (size_t)kWarps * 16 * (R + 4) * 4 + (size_t)2 * 16 * (R + 8) * 2;
+    if (smem > 48 * 1024) {
+      const cudaError_t e = allow_smem(lora_row16_kernel<R, SILU>, (int)smem);
+      if (e != cudaSuccess) return e;
+    }
+    SQ_LAUNCH((lora_row16_kernel<R, SILU>), dim3(p.max_tiles, 1, C), dim3(kThreads), smem, s, C, p);
+    return cudaGetLastError();
+  }
+  cudaError_t e = allow_smem(lora_shrink128_kernel<R>, Shrink128<R>::kSmem);
+  if (e != cudaSuccess) return e;
+  SQ_LAUNCH(lora_shrink128_kernel<R>, dim3(p.max_tiles, 1, C), dim3(kThreads), (size_t)Shrink128<R>::kSmem, s, C, p);
+  using TC = Expand128<R, SILU>;
+  e = allow_smem(lora_expand128_kernel<R, SILU>, TC::kSmem);
+  if (e != cudaSuccess) return e;
+  // runs of units: about three CTAs per resident one, so that the last ones level out
+  const int units = (p.N + 64 * TC::G - 1) / (64 * TC::G);
+  int wave = 3;
+  if (const char* ev = getenv("LORA_U")) wave = atoi(ev);
+  long long run = (long long)p.max_tiles * units / ((long long)wave * TC::kCtas * num_sms);
+  run = run < 4 ? 4 : run > 64 ? 64 : run;
+  LoraParams q = p;
+  q.units = (int)run;
+  SQ_LAUNCH((lora_expand128_kernel<R, SILU>), dim3((units + q.units - 1) / q.units, p.max_tiles), dim3(kThreads),
+            (size_t)TC::kSmem, s, 1, q);
   return cudaGetLastError();
 }
 
 template <int R>
-cudaError_t launch_rank(const LoraParams& p, int C, cudaStream_t s) {
-  return p.silu ? launch_lora<R, true>(p, C, s) : launch_lora<R, false>(p, C, s);
+cudaError_t launch_rank(const LoraParams& p, int C, int num_sms, cudaStream_t s) {
+  return p.silu ? launch_lora<R, true>(p, C, num_sms, s) : launch_lora<R, false>(p, C, num_sms, s);
 }
 
 }  // namespace
 
 cudaError_t lora_plan_launch(const LoraPlanParams& p, cudaStream_t s) {
-  if (p.slots < 1 || p.slots > kLoraMaxSlots || (p.tm != 16 && p.tm != 64)) return cudaErrorInvalidValue;
+  if (p.slots < 1 || p.slots > kLoraMaxSlots || (p.tm != 16 && p.tm != 128)) return cudaErrorInvalidValue;
   const size_t smem = (size_t)(kPlanWarps * (p.slots + 1) + 2 * (p.slots + 2)) * sizeof(int);
   if (smem > 48 * 1024) {
     const cudaError_t e = allow_smem(lora_plan_kernel, (kPlanWarps * (kLoraMaxSlots + 1) + 2 * (kLoraMaxSlots + 2)) * 4);
@@ -647,14 +824,15 @@ cudaError_t lora_plan_launch(const LoraPlanParams& p, cudaStream_t s) {
 
 cudaError_t lora_add_launch(const LoraParams& p, int num_sms, cudaStream_t s) {
   if (p.M == 0 || p.N == 0) return cudaSuccess;
-  if (p.K % 8 || p.N % 8 || (p.silu && p.N % 128) || (p.tm != 16 && p.tm != 64)) return cudaErrorInvalidValue;
+  if (p.K % 8 || p.N % 8 || (p.silu && p.N % 128) || (p.tm != 16 && p.tm != 128)) return cudaErrorInvalidValue;
   int C = 8;
   while (C > 1 && p.max_tiles * C > 4 * num_sms) C >>= 1;
+  if (const char* e = getenv("LORA_C")) C = atoi(e);
   switch (p.R) {
-    case 16: return launch_rank<16>(p, C, s);
-    case 32: return launch_rank<32>(p, C, s);
-    case 64: return launch_rank<64>(p, C, s);
-    case 128: return launch_rank<128>(p, C, s);
+    case 16: return launch_rank<16>(p, C, num_sms, s);
+    case 32: return launch_rank<32>(p, C, num_sms, s);
+    case 64: return launch_rank<64>(p, C, num_sms, s);
+    case 128: return launch_rank<128>(p, C, num_sms, s);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -176,7 +176,7 @@ void lora_plan(torch::Tensor row_slot, int64_t slots, int64_t tm, torch::Tensor 
   const auto dev = cuda_device(row_slot, "row_slots");
   const int64_t M = row_slot.numel();
   TORCH_CHECK(slots >= 1 && slots <= sq::kLoraMaxSlots, "1..", str(sq::kLoraMaxSlots), " adapter slots, not ", str(slots));
-  TORCH_CHECK(tm == 16 || tm == 64, "tile rows must be 16 or 64");
+  TORCH_CHECK(tm == 16 || tm == 128, "tile rows must be 16 or 128");
   TORCH_CHECK(M <= (1 << 24), "too many rows");
   sq::LoraPlanParams p{};
   p.row_slot = arr<int>(row_slot, "row_slots", I32, dev, 0);
@@ -212,7 +212,7 @@ bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
 
 void lora_add(torch::Tensor x, torch::Tensor a, torch::Tensor b, torch::Tensor rank, torch::Tensor scale,
               torch::Tensor y, torch::Tensor out, torch::Tensor order, torch::Tensor tiles, torch::Tensor num_tiles,
-              int64_t tm, int64_t slots, int64_t max_tiles, bool silu) {
+              int64_t tm, int64_t slots, int64_t max_tiles, bool silu, torch::Tensor status) {
   const auto dev = cuda_device(x, "x");
   check(a, "pool a", BF16, dev);
   check(b, "pool b", BF16, dev);
@@ -249,8 +249,14 @@ void lora_add(torch::Tensor x, torch::Tensor a, torch::Tensor b, torch::Tensor r
   p.tm = (int)tm;
   p.max_tiles = (int)max_tiles;
   p.silu = silu;
+  p.status = arr<int>(status, "status", I32, dev, 1);
   if (M == 0) return;
   const c10::cuda::CUDAGuard g(dev);
+  torch::Tensor h;  // from the caching allocator, in this stream's order: calls never share it
+  if (tm != 16) {
+    h = torch::empty({M, 2, R}, x.options());
+    p.h = reinterpret_cast<__nv_bfloat16*>(h.data_ptr());
+  }
   ok(sq::lora_add_launch(p, sms(), stream()), "lora_add");
 }
 

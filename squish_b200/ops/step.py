@@ -12,6 +12,13 @@ import torch
 from .._ext import native
 from .kernels import Int4Weight, Workspace, _count, w4a16_linear, workspace
 
+def _status(ws: Workspace | None, t: torch.Tensor, name: str) -> torch.Tensor:
+    """Status word of the given workspace, or of the one of the tensor's device."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    return (ws or workspace(t.device)).status
+
+
 LAYOUT_TILE = 32  # queries per attention tile (models.decoder.prefill_tiles)
 
 
@@ -71,9 +78,8 @@ def step_layout(ctx_len: torch.Tensor, q_len: torch.Tensor, block_tables: torch.
     b = ctx_len.numel()
     if b != out.seqs:
         out._narrow(b)
-    ws = ws or workspace(ctx_len.device)
     native().step_layout(ctx_len, q_len, block_tables, free_pages, page_size, out.tile, out.buf, out.max_seqs,
-                         out.max_tokens, out.max_tiles, ws.status)
+                         out.max_tokens, out.max_tiles, _status(ws, ctx_len, "ctx_len"))
     _count()
     return out
 
@@ -203,9 +209,9 @@ class LoraPlan:
     projection of the step."""
 
     def __init__(self, rows: int, slots: int, device):
-        # tiles of 16 rows while adapters have few rows each, of 64 for prefill: a tile reads its
+        # tiles of 16 rows while adapters have few rows each, of 128 for prefill: a tile reads its
         # adapter once, so wider tiles re-read less (from L2) but leave more of themselves empty
-        self.tile_rows = 16 if rows <= 512 else 64
+        self.tile_rows = 16 if rows <= 512 else 128
         self.rows, self.slots = rows, slots
         self.max_tiles = -(-rows // self.tile_rows) + min(slots + 1, rows)
         i32 = dict(dtype=torch.int32, device=device)
@@ -224,21 +230,21 @@ def lora_plan(row_slots: torch.Tensor, slots: int, out: LoraPlan | None = None,
         out = LoraPlan(m, slots, row_slots.device)
     elif out.rows != m or out.slots != slots:
         raise ValueError(f"a plan for {out.rows} rows and {out.slots} slots, not {m} and {slots}")
-    ws = ws or workspace(row_slots.device)
-    native().lora_plan(row_slots, slots, out.tile_rows, out.order, out.tiles, out.num_tiles, ws.status)
+    native().lora_plan(row_slots, slots, out.tile_rows, out.order, out.tiles, out.num_tiles,
+                       _status(ws, row_slots, "row_slots"))
     _count()
     return out
 
 
 def lora_add(x: torch.Tensor, pool: LoraPool, plan: LoraPlan, y: torch.Tensor, out: torch.Tensor | None = None,
-             silu_mul: bool = False) -> torch.Tensor:
+             silu_mul: bool = False, ws: Workspace | None = None) -> torch.Tensor:
     """out[t] = y[t] + scale_s B_s (A_s x[t]) for row t with adapter slot s, out[t] = y[t] without
     one; x [M, K], y [M, N] bf16. ``out`` may be y itself. With ``silu_mul`` the columns of y are
     interleaved gate/up blocks of 64 and out = silu(gate) * up has N/2 columns."""
     if out is None:
         out = torch.empty((x.shape[0], pool.n // 2 if silu_mul else pool.n), dtype=torch.bfloat16, device=x.device)
     native().lora_add(x, pool.a, pool.b, pool.rank, pool.scale, y, out, plan.order, plan.tiles, plan.num_tiles,
-                      plan.tile_rows, plan.slots, plan.max_tiles, silu_mul)
+                      plan.tile_rows, plan.slots, plan.max_tiles, silu_mul, _status(ws, x, "x"))
     _count()
     return out
 
@@ -249,8 +255,8 @@ def lora_linear(x: torch.Tensor, w: Int4Weight, pool: LoraPool, plan: LoraPlan, 
     """:func:`w4a16_linear` with the rows' adapters added (before the SiLU*up epilogue)."""
     if not silu_mul:
         y = w4a16_linear(x, w, out=out, residual=residual, ws=ws)
-        return lora_add(x, pool, plan, y, out=y)
+        return lora_add(x, pool, plan, y, out=y, ws=ws)
     if residual is not None:
         raise ValueError("a residual cannot follow the SiLU*up epilogue")
     y = w4a16_linear(x, w, ws=ws)
-    return lora_add(x, pool, plan, y, out=out, silu_mul=True)
+    return lora_add(x, pool, plan, y, out=out, silu_mul=True, ws=ws)
