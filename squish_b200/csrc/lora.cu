@@ -568,11 +568,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink128_kernel(const LoraP
 
 template <int R, bool SILU>
 struct Expand128 {
-  static constexpr int G = SILU ? 2 : 1;
+  // 64-column halves of a unit: gate and up, or two where they fit (a row's share of a unit is then 256
+  // contiguous bytes, which the memory serves faster than 128)
+  static constexpr int G = SILU || R <= 32 ? 2 : 1;
   // h: [128 rows][upper | lower] in 128-byte rows; B: [64 G columns][ranks] likewise, but up to rank 32
-  // gate and up share a row (64 bytes each)
+  // the two halves share a row (64 bytes each)
   static constexpr int kA = 128 * 128 * (R >= 64 ? R / 32 : 1);
-  static constexpr bool kPair = SILU && R <= 32;
+  static constexpr bool kPair = R <= 32;
   static constexpr int kBRows = kPair ? 64 : 64 * G;
   static constexpr int kB = kBRows * 128 * (R >= 64 ? R / 64 : 1);
   static constexpr int kStage = G * 128 * 128 + kB;
@@ -587,6 +589,7 @@ template <int R, bool SILU>
 __global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expand128_kernel(const LoraParams p) {
   using TC = Expand128<R, SILU>;
   constexpr int S = TC::S, G = TC::G;
+  constexpr int OQ = SILU ? 1 : G;  // 64-column halves of the output of a unit
   static_assert(S >= 2 && TC::kStage % 1024 == 0, "ring");
   // The launch before this one is the shrink, which lets this one start once everything before it is
   // complete: the plan, y and B may be read at once, h after the wait.
@@ -632,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expa
     const int r = rows[lr + 32 * j];
     on |= (r >= 0 ? 1u : 0u) << j;
     py[j] = p.y + (r < 0 ? 0 : r) * p.ldy + (long long)u0 * 64 * G + lc * 8;
-    po[j] = p.out + (r < 0 ? 0 : r) * p.ldo + (long long)u0 * 64 + lc * 8;
+    po[j] = p.out + (r < 0 ? 0 : r) * p.ldo + (long long)u0 * 64 * OQ + lc * 8;
   }
   constexpr int CH = R / 8;          // 16-byte pieces of a B row
   constexpr int BN = kThreads / CH;  // B rows per pass
@@ -644,12 +647,13 @@ __global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expa
     uint8_t* st = ring + wr * TC::kStage;
     wr = wr == S - 1 ? 0 : wr + 1;
     if (i < n2) {
-      const bool in = SILU || col + lc * 8 < p.N;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
 #pragma unroll
-        for (int q = 0; q < G; ++q)
+        for (int q = 0; q < G; ++q) {
+          const bool in = SILU || col + q * 64 + lc * 8 < p.N;
           cp16(st + q * 16384 + so + j * 4096, in ? py[j] + q * 64 : p.y, in && ((on >> j) & 1u));
+        }
         py[j] += 64 * G;
       }
       if (bc * 8 < live) {
@@ -714,57 +718,59 @@ __global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expa
       mbar_wait(&done, (uint32_t)i & 1u, p.status, SQ_ERR_TIMEOUT_ACC);
       tc_fence_after();
     }
-    // 32 output columns of the thread's row, 16 at a time, in place of y
+    // 32 output columns of each half of the thread's row, 16 at a time, in place of y
 #pragma unroll
-    for (int c = 0; c < 32; c += 16) {
-      const int c0 = hf * 32 + c;
-      uint32_t v[G][16];
-      if (live > 0) {
+    for (int oq = 0; oq < OQ; ++oq) {
 #pragma unroll
-        for (int q = 0; q < G; ++q) tmem_ld16(lanes + q * 64 + c0, v[q]);
-        tmem_wait_ld();
-      } else {
+      for (int c = 0; c < 32; c += 16) {
+        const int c0 = hf * 32 + c;
+        uint32_t v[2][16];  // product (SiLU*up: of the gate and of the up columns)
+        if (live > 0) {
+          tmem_ld16(lanes + oq * 64 + c0, v[0]);
+          if (SILU) tmem_ld16(lanes + 64 + c0, v[1]);
+          tmem_wait_ld();
+        } else {
 #pragma unroll
-        for (int q = 0; q < G; ++q)
-#pragma unroll
-          for (int k = 0; k < 16; ++k) v[q][k] = 0u;
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4* at = reinterpret_cast<uint4*>(st + sw(row, c0 / 8 + h));
-        const uint4 y = *at;
-        const uint32_t yw[4] = {y.x, y.y, y.z, y.w};
-        uint32_t uw[4] = {0, 0, 0, 0};
-        if (SILU) {
-          const uint4 x = *reinterpret_cast<const uint4*>(st + 16384 + sw(row, c0 / 8 + h));
-          uw[0] = x.x;
-          uw[1] = x.y;
-          uw[2] = x.z;
-          uw[3] = x.w;
+          for (int k = 0; k < 16; ++k) v[0][k] = v[1][k] = 0u;
         }
-        uint32_t o[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float f0 = lo_f(yw[k]) + __uint_as_float(v[0][8 * h + 2 * k]);
-          float f1 = hi_f(yw[k]) + __uint_as_float(v[0][8 * h + 2 * k + 1]);
+        for (int h = 0; h < 2; ++h) {
+          uint4* at = reinterpret_cast<uint4*>(st + oq * 16384 + sw(row, c0 / 8 + h));
+          const uint4 y = *at;
+          const uint32_t yw[4] = {y.x, y.y, y.z, y.w};
+          uint32_t uw[4] = {0, 0, 0, 0};
           if (SILU) {
-            f0 = silu_mul(f0, lo_f(uw[k]) + __uint_as_float(v[G - 1][8 * h + 2 * k]));
-            f1 = silu_mul(f1, hi_f(uw[k]) + __uint_as_float(v[G - 1][8 * h + 2 * k + 1]));
+            const uint4 x = *reinterpret_cast<const uint4*>(st + 16384 + sw(row, c0 / 8 + h));
+            uw[0] = x.x;
+            uw[1] = x.y;
+            uw[2] = x.z;
+            uw[3] = x.w;
           }
-          o[k] = pack_bf16(f0, f1);
+          uint32_t o[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float f0 = lo_f(yw[k]) + __uint_as_float(v[0][8 * h + 2 * k]);
+            float f1 = hi_f(yw[k]) + __uint_as_float(v[0][8 * h + 2 * k + 1]);
+            if (SILU) {
+              f0 = silu_mul(f0, lo_f(uw[k]) + __uint_as_float(v[1][8 * h + 2 * k]));
+              f1 = silu_mul(f1, hi_f(uw[k]) + __uint_as_float(v[1][8 * h + 2 * k + 1]));
+            }
+            o[k] = pack_bf16(f0, f1);
+          }
+          *at = make_uint4(o[0], o[1], o[2], o[3]);
         }
-        *at = make_uint4(o[0], o[1], o[2], o[3]);
       }
     }
     tc_fence_before();
     __syncthreads();
-    if (SILU || (u0 + i) * 64 + lc * 8 < p.N) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if ((on >> j) & 1u) *reinterpret_cast<uint4*>(po[j]) = *reinterpret_cast<const uint4*>(st + so + j * 4096);
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int oq = 0; oq < OQ; ++oq)
+        if (((on >> j) & 1u) && (SILU || (u0 + i) * 64 * OQ + oq * 64 + lc * 8 < p.N))
+          *reinterpret_cast<uint4*>(po[j] + oq * 64) = *reinterpret_cast<const uint4*>(st + oq * 16384 + so + j * 4096);
+      po[j] += 64 * OQ;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) po[j] += 64;
   }
   cp_wait<0>();
   __syncthreads();
@@ -793,10 +799,8 @@ cudaError_t launch_lora(const LoraParams& p, int C, int num_sms, cudaStream_t s)
   if (e != cudaSuccess) return e;
   // runs of units: about three CTAs per resident one, so that the last ones level out
   const int units = (p.N + 64 * TC::G - 1) / (64 * TC::G);
-  int wave = 3;
-  if (const char* ev = getenv("LORA_U")) wave = atoi(ev);
-  long long run = (long long)p.max_tiles * units / ((long long)wave * TC::kCtas * num_sms);
-  run = run < 4 ? 4 : run > 64 ? 64 : run;
+  long long run = (long long)p.max_tiles * units / (3ll * TC::kCtas * num_sms);
+  run = run < 2 ? 2 : run > 64 ? 64 : run;
   LoraParams q = p;
   q.units = (int)run;
   SQ_LAUNCH((lora_expand128_kernel<R, SILU>), dim3((units + q.units - 1) / q.units, p.max_tiles), dim3(kThreads),
@@ -825,9 +829,10 @@ cudaError_t lora_plan_launch(const LoraPlanParams& p, cudaStream_t s) {
 cudaError_t lora_add_launch(const LoraParams& p, int num_sms, cudaStream_t s) {
   if (p.M == 0 || p.N == 0) return cudaSuccess;
   if (p.K % 8 || p.N % 8 || (p.silu && p.N % 128) || (p.tm != 16 && p.tm != 128)) return cudaErrorInvalidValue;
+  // CTAs per tile (K split over them): more while few tiles leave SMs idle. Measured with 2, 4, 8: 33
+  // tiles at most, K 3584: 64, 60, 58 us; 82 tiles, K 4096: 65, 61, 65 us; 72 tiles, K 2048: 40, 38, 45 us.
   int C = 8;
-  while (C > 1 && p.max_tiles * C > 4 * num_sms) C >>= 1;
-  if (const char* e = getenv("LORA_C")) C = atoi(e);
+  while (C > 1 && p.max_tiles * C > (p.tm == 16 ? 4 : 3) * num_sms) C >>= 1;
   switch (p.R) {
     case 16: return launch_rank<16>(p, C, num_sms, s);
     case 32: return launch_rank<32>(p, C, num_sms, s);
