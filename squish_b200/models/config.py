@@ -38,6 +38,13 @@ class ModelConfig:
     norm_topk_prob: bool = True
     expert_offset: int = 0       # expert parallelism: this rank holds experts
     num_local_experts: int = 0   # [expert_offset, expert_offset + num_local_experts) (0 = all)
+    # router (ops.moe_route_scored): scores, expert groups of which the best are open, weight scale; a
+    # per-expert choice bias is the checkpoint tensor mlp.gate.bias
+    router_score: str = "softmax"      # "softmax" | "sigmoid"
+    router_groups: int = 1
+    router_top_groups: int = 0         # open groups (0 = all)
+    router_group_score: str = "max"    # a group's rank: its best choice score, or "top2": the sum of two
+    router_scale: float = 1.0
     rope_scaling: dict | None = None
     bos_token_id: int = 1
     eos_token_id: int = 2
@@ -45,6 +52,11 @@ class ModelConfig:
     @property
     def is_moe(self) -> bool:
         return self.num_experts > 0
+
+    @property
+    def plain_router(self) -> bool:
+        """Softmax over all experts, top-k, no scale: the routing of moe_route."""
+        return self.router_score == "softmax" and self.router_groups == 1 and self.router_scale == 1.0
 
     @property
     def q_size(self) -> int:
@@ -179,6 +191,11 @@ def from_hf_config(path: str) -> ModelConfig:
         num_experts_per_tok=d.get("num_experts_per_tok", 0) or 0,
         moe_intermediate_size=d.get("moe_intermediate_size", 0) or 0,
         norm_topk_prob=d.get("norm_topk_prob", True),
+        router_score=d.get("scoring_func") or "softmax",
+        router_groups=d.get("n_group") or 1,
+        router_top_groups=d.get("topk_group") or 0,
+        router_group_score="top2" if d.get("topk_method") == "noaux_tc" else "max",
+        router_scale=d.get("routed_scaling_factor") or 1.0,
         rope_scaling=d.get("rope_scaling"),
         bos_token_id=d.get("bos_token_id", 1) or 1,
         eos_token_id=eos,
@@ -212,6 +229,11 @@ def to_hf_config(cfg: ModelConfig) -> dict:
         d.update(num_experts=cfg.num_experts, num_experts_per_tok=cfg.num_experts_per_tok,
                  moe_intermediate_size=cfg.moe_intermediate_size, norm_topk_prob=cfg.norm_topk_prob,
                  decoder_sparse_step=1, mlp_only_layers=[])
+        if not cfg.plain_router:
+            d.update(scoring_func=cfg.router_score, n_group=cfg.router_groups,
+                     topk_group=cfg.router_top_groups or cfg.router_groups, routed_scaling_factor=cfg.router_scale)
+            if cfg.router_group_score == "top2":
+                d["topk_method"] = "noaux_tc"
     if cfg.rope_scaling:
         d["rope_scaling"] = cfg.rope_scaling
     return d

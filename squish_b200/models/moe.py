@@ -1,5 +1,6 @@
-"""Mixture-of-experts FFN (Qwen3-MoE: softmax router, top-k experts, renormalised weights)
-on the sm_100a kernels.
+"""Mixture-of-experts FFN (Qwen3-MoE: softmax router, top-k experts, renormalised weights;
+or, by the config's router fields and a choice bias in the checkpoint, sigmoid scores, expert
+groups and a weight scale) on the sm_100a kernels.
 
 One step of a layer:
 
@@ -60,8 +61,10 @@ def _interleave(gate, up):
 
 class MoELayer:
     def __init__(self, cfg: ModelConfig, gate_w: torch.Tensor, gate_up: K_.GroupedInt4Weight,
-                 down: K_.GroupedInt4Weight, scratch: MoEScratch | None = None):
+                 down: K_.GroupedInt4Weight, scratch: MoEScratch | None = None,
+                 gate_bias: torch.Tensor | None = None):
         self.cfg = cfg
+        self.gate_bias = gate_bias  # [E] fp32 added to the scores for the choice, or None
         self.gate_w = gate_w  # [E, H] bf16
         self.gate_up = gate_up
         self.down = down
@@ -90,7 +93,18 @@ class MoELayer:
             d = _as_q4a(t[q + "down_proj.weight"], g)
             dn.append(ops.prepare_int4_weight(d.packed, d.scales, d.offsets, d.shape[1], d.group, dev))
         gate_w = t[p + "gate.weight"].data.to(dev, torch.bfloat16).contiguous()
-        return cls(cfg, gate_w, K_.stack_int4_experts(gu), K_.stack_int4_experts(dn), scratch)
+        bias = t[p + "gate.bias"].data.to(dev, torch.float32).contiguous() if p + "gate.bias" in t else None
+        return cls(cfg, gate_w, K_.stack_int4_experts(gu), K_.stack_int4_experts(dn), scratch, bias)
+
+    def route(self, logits: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor) -> None:
+        """Expert ids and weights of the router's logits [T, E], by the config's rules."""
+        c = self.cfg
+        if c.plain_router and self.gate_bias is None:
+            K_.moe_route(logits, self.K, c.norm_topk_prob, ids, weights)
+        else:
+            ops.moe_route_scored(logits, self.K, ids, weights, score=c.router_score, bias=self.gate_bias,
+                                 groups=c.router_groups, top_groups=c.router_top_groups or c.router_groups,
+                                 group_score=c.router_group_score, renorm=c.norm_topk_prob, scale=c.router_scale)
 
     def forward(self, x: torch.Tensor, h: torch.Tensor, ws=None) -> None:
         """h[:T] += MoE(x[:T]) in place."""
@@ -105,7 +119,7 @@ class MoELayer:
         P = K_.moe_padded_rows(T, K, E, bn)
         TK = T * K
         logits = torch.mm(x, self.gate_w.t(), out=sc.logits[:T])
-        K_.moe_route(logits, K, self.cfg.norm_topk_prob, sc.ids[:TK], sc.w[:TK])
+        self.route(logits, sc.ids[:TK], sc.w[:TK])
         if self.offset:
             sc.ids[:TK].sub_(self.offset)  # global -> local expert ids; others fall outside [0, E_local)
         K_.moe_align(sc.ids[:TK], E, bn, sc.sorted_slot[:P], sc.slot_pos[:TK], sc.tile_expert[: P // bn],
@@ -129,6 +143,8 @@ class MoELayer:
         ranks holding its experts, run the local experts over the tp x R received row slots and
         send the weighted sums back to the row owners' reduce-scatter blocks. Returns the
         arrivals per source that the owners' tp_rs_norm_ag waits for."""
+        if not self.cfg.plain_router or self.gate_bias is not None:
+            raise ValueError("the expert all-to-all routes by plain softmax top-k (use tp_mode='nvlink' or 'nccl')")
         sc = self.scratch
         R = comm.sp_rows(T)
         Tr = comm.tp * R

@@ -140,11 +140,7 @@ class ReferenceModel:
             return self._rp(act, w[p + "mlp.down_proj.weight"])
         if self.moe_hook is not None:
             return self.moe_hook(p, x)
-        logits = x @ w[p + "mlp.gate.weight"].T
-        probs = torch.softmax(logits, dim=-1)
-        topv, topi = probs.topk(cfg.num_experts_per_tok, dim=-1)
-        if cfg.norm_topk_prob:
-            topv = topv / topv.sum(-1, keepdim=True)
+        topv, topi = self.route(p, x)
         out = torch.zeros_like(x)
         e0 = cfg.expert_offset
         e1 = e0 + (cfg.num_local_experts or cfg.num_experts)
@@ -159,11 +155,26 @@ class ReferenceModel:
     def route(self, p: str, x: torch.Tensor):
         """(weights, global expert ids) [T, K] of the router of MoE layer ``p``."""
         cfg = self.cfg
-        probs = torch.softmax(x @ self.w[p + "mlp.gate.weight"].T, dim=-1)
-        topv, topi = probs.topk(cfg.num_experts_per_tok, dim=-1)
+        logits = x @ self.w[p + "mlp.gate.weight"].T
+        bias = self.w[p + "mlp.gate.bias"] if p + "mlp.gate.bias" in self.w else None
+        if cfg.plain_router and bias is None:
+            probs = torch.softmax(logits, dim=-1)
+            topv, topi = probs.topk(cfg.num_experts_per_tok, dim=-1)
+        else:
+            probs = torch.sigmoid(logits) if cfg.router_score == "sigmoid" else torch.softmax(logits, dim=-1)
+            choice = probs if bias is None else probs + bias
+            G = cfg.router_groups
+            if G > 1:
+                grp = choice.view(choice.shape[0], G, -1)
+                n = min(2, grp.shape[-1]) if cfg.router_group_score == "top2" else 1
+                best = grp.topk(n, dim=-1).values.sum(-1).topk(cfg.router_top_groups or G, dim=-1).indices
+                closed = torch.ones_like(grp[..., 0], dtype=torch.bool).scatter_(1, best, False)
+                choice = choice.masked_fill(closed.repeat_interleave(grp.shape[-1], dim=1), float("-inf"))
+            topi = choice.topk(cfg.num_experts_per_tok, dim=-1).indices
+            topv = probs.gather(-1, topi)
         if cfg.norm_topk_prob:
             topv = topv / topv.sum(-1, keepdim=True)
-        return topv, topi
+        return (topv if cfg.router_scale == 1.0 else topv * cfg.router_scale), topi
 
     def expert(self, p: str, e: int, xr: torch.Tensor) -> torch.Tensor:
         """Expert ``e`` (global id) of MoE layer ``p`` on one row."""

@@ -32,6 +32,8 @@ class TPCudaRunner(CudaRunner):
         del self.logits
         self.logits = comm.logits_full
         moe = [lw.moe for lw in self.layers if lw.moe is not None]
+        if moe and comm.mode == "sp" and (not self.cfg.plain_router or any(m.gate_bias is not None for m in moe)):
+            raise ValueError("the sequence-parallel mode routes by plain softmax top-k (use tp_mode='nvlink' or 'nccl')")
         if moe and comm.mode == "sp":
             # expert parallelism with the all-to-all: the MoE scratch covers every source's slots
             from ..models.moe import MoEScratch

@@ -129,3 +129,60 @@ def test_reference_forms():
     np.testing.assert_allclose(w[0], s / s.sum())
     ids, _ = route_ref(torch.tensor([[0.0, 3.0, 2.0, 2.0]]), 2, "sigmoid", groups=2, top_groups=1, group_score="top2")
     assert ids.tolist() == [[2, 3]]
+
+
+def _scored_moe():
+    import dataclasses
+
+    from squish_b200.models.config import get_preset
+    from squish_b200.models.weights import QTensor, random_checkpoint
+
+    cfg, q = get_preset("tiny-moe")
+    cfg = dataclasses.replace(cfg, router_score="sigmoid", router_groups=4, router_top_groups=2,
+                              router_group_score="top2", router_scale=2.5)
+    ck = random_checkpoint(cfg, q, seed=3)
+    g = torch.Generator().manual_seed(5)
+    for i in range(cfg.num_layers):
+        ck.tensors[f"model.layers.{i}.mlp.gate.bias"] = QTensor(
+            "dense", (cfg.num_experts,), data=torch.randn(cfg.num_experts, generator=g) * 0.05)
+    return cfg, q, ck
+
+
+def test_scored_router_in_the_reference_model():
+    """The CPU model's router against the 64-bit form, and through the layers."""
+    from squish_b200.models.reference import ReferenceModel
+
+    cfg, _, ck = _scored_moe()
+    ref = ReferenceModel(ck)
+    x = torch.randn(9, cfg.hidden_size, generator=torch.Generator().manual_seed(1))
+    p = "model.layers.0."
+    w, ids = ref.route(p, x)
+    want_i, want_w = route_ref(x @ ref.w[p + "mlp.gate.weight"].T, cfg.num_experts_per_tok, "sigmoid",
+                               ref.w[p + "mlp.gate.bias"], 4, 2, "top2", cfg.norm_topk_prob, 2.5)
+    assert np.array_equal(ids.numpy(), want_i)
+    np.testing.assert_allclose(w.numpy(), want_w, rtol=1e-5)
+    assert torch.isfinite(ref.forward([1, 2, 3], ref.new_cache(), 0)).all()
+
+
+def test_router_config_round_trip(tmp_path):
+    import json
+
+    from squish_b200.models.config import from_hf_config, get_preset, to_hf_config
+
+    cfg, _, _ = _scored_moe()
+    (tmp_path / "config.json").write_text(json.dumps(to_hf_config(cfg)))
+    back = from_hf_config(str(tmp_path))
+    for f in ("router_score", "router_groups", "router_top_groups", "router_group_score", "router_scale"):
+        assert getattr(back, f) == getattr(cfg, f), f
+    assert not back.plain_router
+    plain, _ = get_preset("tiny-moe")
+    assert plain.plain_router and "scoring_func" not in to_hf_config(plain)
+
+
+def test_shards_keep_the_router_bias():
+    from squish_b200.parallel.shard import shard_checkpoint
+
+    cfg, _, ck = _scored_moe()
+    for r in range(2):
+        sh = shard_checkpoint(ck, r, 2)
+        assert sh.config.router_score == "sigmoid" and "model.layers.1.mlp.gate.bias" in sh.tensors

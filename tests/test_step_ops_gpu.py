@@ -721,3 +721,40 @@ def test_layout_drives_the_paged_attention(cuda, pad_tiles):
         ctx = [c + n_ for c, n_ in zip(ctx, q)]
     ops.workspace(cuda).check()
     assert lay.tile_q0.tolist().count(PAD_Q0) >= pad_tiles
+
+
+# ----------------------------------------------------------------------------- in the model
+def test_scored_router_model_matches_the_cpu_model(cuda):
+    """A MoE model with sigmoid scores, a choice bias, expert groups and a weight scale: the layer's
+    routing is the exact one, and the engine (eager and in decode graphs) follows the CPU model."""
+    from squish_b200.engine.engine import EngineConfig, LLMEngine
+    from squish_b200.engine.sampling import SamplingParams
+    from squish_b200.models.moe import MoELayer
+    from squish_b200.models.reference import ReferenceModel
+
+    from .test_step_ops_cpu import _scored_moe
+
+    cfg, _, ck = _scored_moe()
+    layer = MoELayer.from_checkpoint(ck, 0, cuda)
+    x = torch.randn(70, cfg.hidden_size, generator=torch.Generator().manual_seed(2)).to(BF)
+    h = torch.zeros(70, cfg.hidden_size, dtype=BF, device=cuda)
+    layer.forward(x.to(cuda), h)
+    logits = torch.mm(x.to(cuda), layer.gate_w.t())
+    n, k = 70 * cfg.num_experts_per_tok, cfg.num_experts_per_tok
+    ids, w = route_ref(logits, k, "sigmoid", layer.gate_bias.cpu(), 4, 2, "top2", cfg.norm_topk_prob, 2.5)
+    assert np.array_equal(layer.scratch.ids[:n].view(70, k).cpu().numpy(), ids)
+    np.testing.assert_allclose(layer.scratch.w[:n].view(70, k).cpu().numpy(), w, rtol=2.0**-18)
+    assert h.abs().max() > 0
+
+    ref = ReferenceModel(ck)
+    prompt = np.random.default_rng(5).integers(0, cfg.vocab_size, 40).tolist()
+    ref_logits = ref.forward(prompt, ref.new_cache(), 0)[-1]
+    eng = LLMEngine.from_checkpoint(_scored_moe()[2], cuda, EngineConfig(max_num_seqs=4, max_num_batched_tokens=64,
+                                                                         max_model_len=256, num_pages=64))
+    eng.add_request(prompt, SamplingParams(max_tokens=1, ignore_eos=True))
+    eng.step()
+    cos = torch.nn.functional.cosine_similarity(eng.runner.logits[0].float().cpu(), ref_logits, dim=0)
+    assert cos > 0.99, cos
+    outs = eng.generate([prompt, prompt[:17]], SamplingParams(max_tokens=6, ignore_eos=True))
+    assert [len(o) for o in outs] == [6, 6]
+    eng.runner.ws.check()
