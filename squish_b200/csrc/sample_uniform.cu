@@ -67,6 +67,24 @@ struct Shared {
   int r_bits, r_rank;
 };
 
+// e^x for x <= 0: x = k ln 2 + r, |r| <= ln 2 / 2 (ln 2 in two parts, Cody and Waite), the Taylor
+// polynomial of degree 13 (remainder 4e-18) evaluated in pairs (Estrin), times 2^k; 0 below 2^-1021.
+// Within 4 ulp. The chain is 11 operations where one after another it would be 20: the
+// exponentials are waited for, not many.
+__device__ __forceinline__ double exp_neg(double x) {
+  const double kx = fma(x, 1.4426950408889634, 6755399441055744.0);  // 1.5 * 2^52: rounds to an integer
+  const double k = kx - 6755399441055744.0;
+  const double r = fma(k, -1.9082149292705877e-10, fma(k, -6.93147180369123816490e-01, x));
+  const double r2 = r * r, r4 = r2 * r2, r8 = r4 * r4;
+  const double p01 = 1.0 + r, p23 = fma(r, 1.0 / 6, 0.5), p45 = fma(r, 1.0 / 120, 1.0 / 24),
+               p67 = fma(r, 1.0 / 5040, 1.0 / 720), p89 = fma(r, 1.0 / 362880, 1.0 / 40320),
+               pab = fma(r, 1.0 / 39916800, 1.0 / 3628800), pcd = fma(r, 1.0 / 6227020800.0, 1.0 / 479001600);
+  const double q0 = fma(p23, r2, p01), q1 = fma(p67, r2, p45), q2 = fma(pab, r2, p89);
+  const double e = fma(fma(pcd, r4, q2), r8, fma(q1, r4, q0));
+  if (!(x > -707.0)) return 0.0;
+  return e * __hiloint2double((1023 + __double2loint(kx)) << 20, 0);
+}
+
 __device__ __forceinline__ double bf16_value(int bits) { return (double)__uint_as_float((unsigned)bits << 16); }
 
 // bf16 bits of bin j: the main bins (win < 0) or window `win`, both in descending order of value
@@ -198,7 +216,7 @@ __device__ double walk(const Rules& rule, At at, int j0, int per, int win, doubl
     const int c = at(i);
     if (c <= 0) continue;
     const int b = bin_bits(j0 + i, win);
-    const double w = exp(rule.logw(b));
+    const double w = exp_neg(rule.logw(b));
     const int t = rule.keep(c, w, m, k0);
     if (t > 0 && bits != nullptr && (m <= target || *bits < 0)) {
       *bits = b;
@@ -227,14 +245,14 @@ __device__ double warp_walk(const Rules& rule, Bin bin, Cnt count, int first, in
       const int j = bin(first + e + lane);
       b = bin_bits(j, -1);
       c = count(j);
-      w = exp(rule.logw(b));
+      w = exp_neg(rule.logw(b));
     }
     double im = (double)c * w;
-    long long in = c;
+    int in = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double a = __shfl_up_sync(0xffffffffu, im, o);
-      const long long d = __shfl_up_sync(0xffffffffu, in, o);
+      const int d = __shfl_up_sync(0xffffffffu, in, o);
       if (lane >= o) {
         im += a;
         in += d;
@@ -290,16 +308,26 @@ __device__ __forceinline__ void block_prefix(Shared& sh, int turn, double mass, 
     sh.cnt[warp] = in;
   }
   __syncthreads();
-  tm = 0.0;
-  tn = 0;
+  // the warps' sums: lane w takes warp w (fp64 additions one after another would be the longest wait here)
+  static_assert(kWarps == 16, "one lane per warp sum");
+  im = sh.mass[turn][lane & 15];
+  in = sh.cnt[lane & 15];
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w == warp) {
-      em += tm;
-      en += tn;
+  for (int o = 1; o < 16; o <<= 1) {
+    const double a = __shfl_up_sync(0xffffffffu, im, o, 16);
+    const int b = __shfl_up_sync(0xffffffffu, in, o, 16);
+    if ((lane & 15) >= o) {
+      im += a;
+      in += b;
     }
-    tm += sh.mass[turn][w];
-    tn += sh.cnt[w];
+  }
+  tm = __shfl_sync(0xffffffffu, im, 15);
+  tn = __shfl_sync(0xffffffffu, in, 15);
+  const double bm = __shfl_sync(0xffffffffu, im, (warp + 15) & 15);
+  const int bn = __shfl_sync(0xffffffffu, in, (warp + 15) & 15);
+  if (warp > 0) {
+    em += bm;
+    en += bn;
   }
 }
 __device__ __forceinline__ int block_min(Shared& sh, int turn, int v) {
@@ -315,9 +343,9 @@ __device__ __forceinline__ double block_sum(Shared& sh, int turn, double s) {
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) sh.mass[turn][threadIdx.x >> 5] = s;
   __syncthreads();
-  s = 0.0;
+  s = sh.mass[turn][threadIdx.x & 15];
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) s += sh.mass[turn][w];
+  for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
 
@@ -392,6 +420,11 @@ __device__ __forceinline__ void find_token(const SampleUniformParams& p, int row
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       const int own = __popc(m[q]);
+      const int here = __reduce_add_sync(0xffffffffu, own);
+      if (want >= here) {
+        want -= here;
+        continue;
+      }
       int inc = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -399,8 +432,7 @@ __device__ __forceinline__ void find_token(const SampleUniformParams& p, int row
         if (lane >= o) inc += c;
       }
       if (want >= inc - own && want < inc) p.out_tokens[row] = sl.v0 + 8 * (g + 32 * q) + nth_bit(m[q], want - (inc - own));
-      want -= __shfl_sync(0xffffffffu, inc, 31);
-      if (want < 0) return;
+      return;
     }
   }
   const unsigned tm = __ballot_sync(0xffffffffu, lane < sl.tail && match1(sl.t0 + lane));
@@ -431,7 +463,7 @@ __device__ __noinline__ void any_row(const SampleUniformParams& p, int row, Rule
     n = 0;
     for (int i = 0; i < kPer; ++i) {
       const int c = at(i);
-      if (c > 0) mass += (double)c * exp(rule.logw(bin_bits(j0 + i, win)));
+      if (c > 0) mass += (double)c * exp_neg(rule.logw(bin_bits(j0 + i, win)));
       n += c;
     }
     __syncthreads();
@@ -710,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_uniform_kernel(const Sampl
   for (int e = e0; e < e1; e += 2) {
     const int ja = bin(e), jb = e + 1 < e1 ? bin(e + 1) : ja;
     const int ca = count(ja), cb = e + 1 < e1 ? count(jb) : 0;
-    const double wa = exp(rule.logw(bin_bits(ja, -1))), wb = exp(rule.logw(bin_bits(jb, -1)));
+    const double wa = exp_neg(rule.logw(bin_bits(ja, -1))), wb = exp_neg(rule.logw(bin_bits(jb, -1)));
     if (e == e0) w_hi = wa;
     w_lo = wb;
     n += ca + cb;
@@ -735,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_uniform_kernel(const Sampl
     if (row_first != kNone) rule.vmax = bf16_value(bin_bits(row_first, -1));
     if (tid < C) {
       const int f = sh.in[tid].first;
-      sh.scale[tid] = f != kNone ? exp(rule.logw(bin_bits(f, -1))) : 0.0;
+      sh.scale[tid] = f != kNone ? exp_neg(rule.logw(bin_bits(f, -1))) : 0.0;
     }
     __syncthreads();
     z = 0.0;
