@@ -167,10 +167,20 @@ __device__ __forceinline__ int short_list(const uint32_t (&k)[EPL], int K, float
   return total;
 }
 
-// The K largest of 32 keys (hi, lo), in order; lane kk returns the id of pick kk.
+// fp64 value as an order-preserving pair of words.
+__device__ __forceinline__ void ord64(double v, uint32_t& hi, uint32_t& lo) {
+  unsigned long long u = __double_as_longlong(v + 0.0);
+  u ^= (unsigned long long)((long long)u >> 63) | 0x8000000000000000ull;
+  hi = (uint32_t)(u >> 32);
+  lo = (uint32_t)u;
+}
+
+// The K largest of the lanes' keys (hi, lo; hi = 0: none), in order, the lower lane first among equals:
+// lane kk returns the lane of pick kk, `taken` all of them.
 template <bool kTwo>
-__device__ __forceinline__ int pick_list(uint32_t hi, uint32_t lo, int id, int K, int lane) {
-  int my_id = 0;
+__device__ __forceinline__ int pick_list(uint32_t hi, uint32_t lo, int K, int lane, unsigned& taken) {
+  int src = 0;
+  taken = 0;
   for (int kk = 0; kk < K; ++kk) {
     const uint32_t m = __reduce_max_sync(kFull, hi);
     unsigned w = __ballot_sync(kFull, hi == m);
@@ -178,12 +188,12 @@ __device__ __forceinline__ int pick_list(uint32_t hi, uint32_t lo, int id, int K
       const uint32_t l = __reduce_max_sync(kFull, hi == m ? lo : 0u);
       w &= __ballot_sync(kFull, lo == l);
     }
-    const int win = __ffs(w) - 1;
-    const int picked = __shfl_sync(kFull, id, win);
-    if (lane == kk) my_id = picked;
-    if (lane == win) hi = 0u;
+    w &= 0u - w;
+    taken |= w;
+    if (lane == kk) src = __ffs(w) - 1;
+    if ((w >> lane) & 1u) hi = 0u;
   }
-  return my_id;
+  return src;
 }
 
 // The K largest of all keys, one after another (more picks, or more equal values, than a short list).
@@ -239,35 +249,35 @@ __device__ __forceinline__ double choice64(float x, bool sigmoid, float m, doubl
   return c == c ? c : (double)kNegInf;
 }
 
-// Open groups by exact scores (rows whose fp32 group scores lie too close).
+// Open groups by exact scores (rows whose fp32 group scores lie too close). g1, g2: the fp32 best
+// values of group `lane` (choice values; without a bias the logits, which are exact). With a bias only
+// the values that may be a group's best (two) within the error are computed exactly.
 template <int EPL>
-__device__ __noinline__ unsigned open_groups64(const float (&x)[EPL], const float* bias, bool sigmoid, float m,
-                                               double inv_z, const Shape& sh, int lane, double* buf) {
-  double c[EPL], g1, g2;
+__device__ __noinline__ unsigned open_groups64(const float (&x)[EPL], const float (&c)[EPL], float g1, float g2,
+                                               float tol, const float* bias, bool sigmoid, float m, double inv_z,
+                                               const Shape& sh, int lane, double* buf) {
+  const bool two = sh.top2 && sh.gsize > 1;
+  double a = g1, b = g2;
+  if (bias == nullptr) {
+    a = choice64(g1, sigmoid, m, inv_z, 0.f);
+    b = choice64(g2, sigmoid, m, inv_z, 0.f);
+  } else {
+    const float least = (two ? g2 : g1) - tol * (1.f + fabsf(two ? g2 : g1));
+    double v[EPL];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane * EPL + i;
-    c[i] = x[i];
-    if (bias != nullptr) c[i] = e < sh.E ? choice64(x[i], sigmoid, m, inv_z, bias[e]) : (double)kNegInf;
-  }
-  group_top2<EPL, double>(c, sh, lane, buf, g1, g2);
-  double g = g1;
-  if (sh.top2 && sh.gsize > 1) {
-    if (bias == nullptr) {
-      g1 = choice64((float)g1, sigmoid, m, inv_z, 0.f);
-      g2 = choice64((float)g2, sigmoid, m, inv_z, 0.f);
+    for (int i = 0; i < EPL; ++i) {
+      const int e = lane * EPL + i;
+      const float t = __shfl_sync(kFull, least, min(e / sh.gsize, 31));
+      v[i] = (double)kNegInf;
+      if (e < sh.E && !(c[i] < t)) v[i] = choice64(x[i], sigmoid, m, inv_z, bias[e]);
     }
-    g = g1 + g2;
+    group_top2<EPL, double>(v, sh, lane, buf, a, b);
   }
-  bool taken = lane >= sh.groups;
-  unsigned open = 0;
-  for (int t = 0; t < sh.top_groups; ++t) {
-    double v = g;
-    int i = taken ? 0x7fffffff : lane;
-    argmax64(v, i);
-    open |= 1u << i;
-    if (lane == i) taken = true;
-  }
+  uint32_t hi = 0u, lo = 0u;
+  const double g = two ? a + b : a;
+  if (lane < sh.groups) ord64(g == g ? g : (double)kNegInf, hi, lo);
+  unsigned open;
+  pick_list<true>(hi, lo, sh.top_groups, lane, open);
   return open;
 }
 
@@ -356,10 +366,11 @@ __global__ void __launch_bounds__(kWarps * 32) route_scored_kernel(const RouteSc
     for (int o = 16; o; o >>= 1) z64 += __shfl_xor_sync(kFull, z64, o);
     inv_z64 = z64 > 0.0 ? 1.0 / z64 : 0.0;
   }
-  // fp32 choice values. A score (absolute value <= 1) is off by less than 4e-7 (argument rounded by
-  // 2^-24 of itself, exponential 2 ulp, reciprocal 1 ulp), adding the bias rounds by 2^-24 of the sum:
-  // 2e-6 (1 + |c|) is more than the error of a difference of two, or of two sums of two.
-  constexpr float kTol = 2e-6f;
+  // fp32 choice values. A score (absolute value <= 1) is off by less than 2e-7 (argument rounded by
+  // 2^-24 of itself, exponential 2 ulp, reciprocal 1 ulp: times s (1 - s), 2e-7), adding the bias rounds
+  // by 2^-24 of the sum. A difference of two sums of two is off by at most 4 (2e-7 + 6e-8 |c|) + 2 * 6e-8
+  // |sum| < 1e-6 (1 + |sum|), one of two values by half as much.
+  constexpr float kTol = 1e-6f;
   float c[EPL];
   if (p.bias == nullptr) {
 #pragma unroll
@@ -391,16 +402,15 @@ __global__ void __launch_bounds__(kWarps * 32) route_scored_kernel(const RouteSc
     g = g1;
     if (p.bias != nullptr) tol = kTol;
     if (sh.top2 && sh.gsize > 1) {
-      if (p.bias == nullptr) {
-        g1 = g1 == kNegInf ? 0.f : sigm ? sigmoid_fast(g1) : (g1 == m ? 1.f : exp_fast(g1 - m));
-        g2 = g2 == kNegInf ? 0.f : sigm ? sigmoid_fast(g2) : (g2 == m ? 1.f : exp_fast(g2 - m));
-      }
       g = g1 + g2;
+      if (p.bias == nullptr)
+        g = (g1 == kNegInf ? 0.f : sigm ? sigmoid_fast(g1) : (g1 == m ? 1.f : exp_fast(g1 - m))) +
+            (g2 == kNegInf ? 0.f : sigm ? sigmoid_fast(g2) : (g2 == m ? 1.f : exp_fast(g2 - m)));
       tol = kTol;
     }
     bool sure;
     open = open_groups32(g, sh, lane, tol, sure);
-    if (!sure) open = open_groups64<EPL>(x, p.bias, sigm, m, inv_z64, sh, lane, buf);
+    if (!sure) open = open_groups64<EPL>(x, c, g1, g2, kTol, p.bias, sigm, m, inv_z64, sh, lane, buf);
   }
   uint32_t k[EPL];
   unsigned live = 0;
@@ -421,30 +431,40 @@ __global__ void __launch_bounds__(kWarps * 32) route_scored_kernel(const RouteSc
   }
   int my_id, listed = 33;
   uint2 my;
+  float xi = kNegInf, si = -1.f;  // pick `lane`: its logit, its score where it is at hand
   if (sh.K <= kListK) listed = short_list<EPL>(k, sh.K, p.bias == nullptr ? 0.f : kTol, lane, cand[warp], my);
-  if (p.bias == nullptr) {
-    my_id = listed <= 32 ? pick_list<false>(my.x, 0u, (int)my.y, sh.K, lane) : pick_all<EPL>(k, sh.K, lane);
-  } else if (listed <= 32) {
-    uint32_t hi = 0u, lo = 0u;
-    if (lane < listed) {
-      const float xv = clean(F32 ? lf[my.y] : __bfloat162float(lh[my.y]));
-      unsigned long long u = __double_as_longlong(choice64(xv, sigm, m, inv_z64, __ldg(p.bias + my.y)) + 0.0);
-      u ^= (unsigned long long)((long long)u >> 63) | 0x8000000000000000ull;
-      hi = (uint32_t)(u >> 32);
-      lo = (uint32_t)u;
+  if (listed <= 32) {
+    unsigned taken;
+    float xv = unord32(my.x), sv = 0.f;
+    int src;
+    if (p.bias == nullptr) {
+      src = pick_list<false>(my.x, 0u, sh.K, lane, taken);
+    } else {
+      uint32_t hi = 0u, lo = 0u;
+      if (lane < listed) {
+        xv = clean(F32 ? lf[my.y] : __bfloat162float(lh[my.y]));
+        const double s64 = xv == kNegInf ? 0.0 : score64(xv, sigm, m, inv_z64), v = s64 + (double)__ldg(p.bias + my.y);
+        ord64(v == v ? v : (double)kNegInf, hi, lo);
+        sv = (float)s64;
+      }
+      src = pick_list<true>(hi, lo, sh.K, lane, taken);
+      if (sigm) si = __shfl_sync(kFull, sv, src);
     }
-    my_id = pick_list<true>(hi, lo, (int)my.y, sh.K, lane);
+    my_id = __shfl_sync(kFull, (int)my.y, src);
+    xi = __shfl_sync(kFull, xv, src);
   } else {
-    my_id = pick_all64<EPL>(x, p.bias, sigm, m, inv_z64, live, sh.K, lane);
+    my_id = p.bias == nullptr ? pick_all<EPL>(k, sh.K, lane)
+                              : pick_all64<EPL>(x, p.bias, sigm, m, inv_z64, live, sh.K, lane);
+    if (lane < sh.K) xi = clean(F32 ? lf[my_id] : __bfloat162float(lh[my_id]));
   }
   // weights: lane k takes pick k, in fp32 with the accurate exponential and divide
   const bool on = lane < sh.K;
-  const float xi = on ? clean(F32 ? lf[my_id] : __bfloat162float(lh[my_id])) : kNegInf;
+  if (!on) xi = kNegInf;
   float s = 0.f;
   if (sigm) {
     if (on) {
       const float ex = expf(-fabsf(xi));
-      s = (xi >= 0.f ? 1.f : ex) / (1.f + ex);
+      s = si >= 0.f ? si : (xi >= 0.f ? 1.f : ex) / (1.f + ex);
     }
   } else {
     // renormalised: relative to the largest pick, the softmax denominator cancels (next to an
