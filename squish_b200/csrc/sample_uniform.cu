@@ -42,7 +42,8 @@ constexpr int kMagLo = 0x3000;   // 2^-31
 constexpr int kMagN = 0x2000;    // .. 2^33
 constexpr int kWindow = 16384;   // bins of a window of the whole key space (four windows)
 constexpr int kNone = 0x7fffffff;
-constexpr int kHist = kBins + 3;  // counters, in whole 16-byte groups
+constexpr int kSpare = kBins + 3;   // 32 spare counters, one per lane, for disallowed values
+constexpr int kHist = kSpare + 32;  // counters, in whole 16-byte groups
 static_assert(kHist % 4 == 0, "histogram size");
 
 // i-th signed value in descending order -> bin (zero is bin kMagN)
@@ -121,13 +122,15 @@ __device__ __forceinline__ void count_window(unsigned bits, int win, int* hist) 
 __device__ __forceinline__ bool main_word(unsigned w) {
   return (((w & 0x7fff7fffu) + 0x50005000u) & 0xe000e000u) == 0x80008000u;  // magnitude >> 12 is 3 or 4
 }
-// Count both values of a word (ok: bit 0 / 1 set = the lower / upper value is allowed).
+// Count both values of a word (ok: bit 0 / 1 set = the lower / upper value is allowed; others go to the
+// lane's spare counter, which costs a select where a branch per value cost twice the row's time).
 template <bool kAll>
 __device__ __forceinline__ void count_word(unsigned w, unsigned ok, int* hist) {
   const unsigned o = (((w << 2) & 0x7ffc7ffcu) | (w & 0x80008000u));  // two byte offsets 4 * main_at
+  const unsigned spare = 4u * (kSpare + (threadIdx.x & 31));
   char* h = reinterpret_cast<char*>(hist);
-  if (kAll || (ok & 1u)) atomicAdd(reinterpret_cast<int*>(h + (o & 0xffffu)), 1);
-  if (kAll || (ok & 2u)) atomicAdd(reinterpret_cast<int*>(h + (o >> 16)), 1);
+  atomicAdd(reinterpret_cast<int*>(h + (kAll || (ok & 1u) ? o & 0xffffu : spare)), 1);
+  atomicAdd(reinterpret_cast<int*>(h + (kAll || (ok & 2u) ? o >> 16 : spare)), 1);
 }
 
 // A row slice: `head` single values, then 16-byte groups of 8, then `tail` single values.
@@ -143,10 +146,8 @@ struct Slice {
   }
   __device__ __forceinline__ unsigned allowed8(int i) const {
     if (mask == nullptr) return 0xffu;
-    const int s = i & 31;
-    unsigned w = mask[i >> 5] >> s;
-    if (s > 24) w |= mask[(i >> 5) + 1] << (32 - s);
-    return w & 0xffu;
+    // bits i .. i + 7: the word of i and that of i + 7 (the same, or the next one)
+    return __funnelshift_r(mask[i >> 5], mask[(i + 7) >> 5], i & 31) & 0xffu;
   }
   __device__ __forceinline__ unsigned bits(int i) const {
     return *reinterpret_cast<const unsigned short*>(row + i);
@@ -551,15 +552,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_uniform_kernel(const Sampl
     if (tid < sl.tail) one(sl.t0 + tid);
     for (int g0 = tid; g0 < sl.nv; g0 += kThreads * U) {
       uint4 v[U];
+      unsigned allow[U];  // (loaded with the values: one wait for both)
 #pragma unroll
       for (int q = 0; q < U; ++q)
-        if (g0 + q * kThreads < sl.nv) v[q] = sl.group(g0 + q * kThreads);
+        if (g0 + q * kThreads < sl.nv) {
+          v[q] = sl.group(g0 + q * kThreads);
+          allow[q] = sl.allowed8(sl.v0 + 8 * (g0 + q * kThreads));
+        }
 #pragma unroll
       for (int q = 0; q < U; ++q) {
         const int g = g0 + q * kThreads;
         if (g >= sl.nv) break;
         const unsigned w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
-        const unsigned ok = sl.allowed8(sl.v0 + 8 * g);
+        const unsigned ok = allow[q];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           unsigned x = w[j];
@@ -613,15 +618,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_uniform_kernel(const Sampl
     if (tid < sl.tail && sl.allowed(sl.t0 + tid)) inside &= count_main(sl.bits(sl.t0 + tid), hist);
     for (int g0 = tid; g0 < sl.nv; g0 += kThreads * U) {
       uint4 v[U];
+      unsigned allow[U];  // (loaded with the values: one wait for both)
 #pragma unroll
       for (int q = 0; q < U; ++q)
-        if (g0 + q * kThreads < sl.nv) v[q] = sl.group(g0 + q * kThreads);
+        if (g0 + q * kThreads < sl.nv) {
+          v[q] = sl.group(g0 + q * kThreads);
+          allow[q] = sl.allowed8(sl.v0 + 8 * (g0 + q * kThreads));
+        }
 #pragma unroll
       for (int q = 0; q < U; ++q) {
         const int g = g0 + q * kThreads;
         if (g >= sl.nv) break;
         const unsigned w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
-        const unsigned ok = sl.allowed8(sl.v0 + 8 * g);
+        const unsigned ok = allow[q];
         if (ok == 0u) continue;
         const bool plain = main_word(w[0]) && main_word(w[1]) && main_word(w[2]) && main_word(w[3]);
         if (plain && ok == 0xffu) {

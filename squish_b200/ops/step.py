@@ -178,6 +178,7 @@ class LoraPool:
         self.b = torch.zeros(slots, n, r, dtype=torch.bfloat16, device=device)
         self.rank = torch.zeros(slots, dtype=torch.int32, device=device)
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
+        self._filled = [0] * slots  # ranks of a slot that may hold something
 
     def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
         """Put an adapter (A [r, K], B [N, r]; ``scale``: usually alpha / r) into a slot, in the
@@ -190,8 +191,10 @@ class LoraPool:
                              f"{tuple(a.shape)} and {tuple(b.shape)}")
         if not 1 <= r <= self.max_rank:
             raise ValueError(f"rank {r} outside 1..{self.max_rank}")
-        self.a[slot, r:].zero_()
-        self.b[slot, :, r:].zero_()
+        if self._filled[slot] > r:  # a smaller rank leaves nothing of the one before it
+            self.a[slot, r:].zero_()
+            self.b[slot, :, r:].zero_()
+        self._filled[slot] = r
         self.a[slot, :r].copy_(a)
         self.b[slot, :, :r].copy_(b)
         self.rank[slot].fill_(r)
