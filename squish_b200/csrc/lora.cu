@@ -4,20 +4,17 @@
 // optionally followed by the SiLU(gate) * up epilogue over [gate 64 | up 64] column blocks.
 //
 // The plan (lora_plan, once per step, shared by every projection) sorts the rows by slot, stable, and
-// cuts them into tiles of at most tm rows of one adapter. One cluster of C CTAs computes a tile in one
-// launch: each CTA takes 1/C of K and computes its share of h = A_s x (tm x R) on the tensor cores,
-// the shares meet through the cluster's shared memory in fp32, and each CTA then takes 1/C of the
-// output columns. x, y and out cross HBM once; h never leaves the cluster.
+// cuts them into tiles of at most tm rows of one adapter: 16 rows for steps of up to 512 rows, where an
+// adapter has few, 128 for larger ones.
 //
 // The work is bound by bytes (y and out dominate): per row and projection 2 r (K + N) flops against
-// 2 (K + 2 N) bytes. Operands go straight from global memory into mma fragments: the order of k
-// within a 32-value step is free as long as both operands agree, so a lane takes 8 consecutive
-// values (16 bytes) of its row, and the columns of four 8-wide tiles are interleaved so that a lane's
-// accumulators are 8 consecutive columns of out (16-byte loads of y, 16-byte stores of out).
+// 2 (K + 2 N) bytes. Up to 512 rows a cluster computes a tile in one launch (lora_row16_kernel, 6 us for
+// one row of a 3584 x 3584 projection); larger steps take two (lora_shrink128_kernel,
+// lora_expand128_kernel).
 //
-// h is held in fp32 and enters the second product as a sum of two bf16 (upper and lower part, 16
-// bits of h): out is rounded once, as the formula would be; one bf16 alone would add an error of
-// 2^-9 |h| per rank to every column. The rank is small, so the second product costs no time.
+// h = scale A_s x is held in fp32 and enters the second product as a sum of two bf16 (upper and lower
+// part, 16 bits of h): out is rounded once, as the formula would be; one bf16 alone would add an error
+// of 2^-9 |h| per rank to every column. The rank is small, so the second product costs no time.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -148,7 +145,7 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
   return g * r * u;
 }
-// y added to the accumulators of 16 rows x 32 columns: a lane's 8 columns of its two rows ...
+// y added to the accumulators of 16 rows x 32 columns: a lane's 8 columns of its two rows.
 __device__ __forceinline__ void add_to(float (&acc)[4][4], uint4 y0, uint4 y1) {
   const uint32_t w0[4] = {y0.x, y0.y, y0.z, y0.w}, w1[4] = {y1.x, y1.y, y1.z, y1.w};
 #pragma unroll
@@ -157,18 +154,6 @@ __device__ __forceinline__ void add_to(float (&acc)[4][4], uint4 y0, uint4 y1) {
     acc[j][1] += hi_f(w0[j]);
     acc[j][2] += lo_f(w1[j]);
     acc[j][3] += hi_f(w1[j]);
-  }
-}
-// ... or as their start, where y is at hand before the products (16 additions and 16 zeros fewer).
-__device__ __forceinline__ void start_from(float (&acc)[4][4], uint4 y0, uint4 y1) {
-  const uint32_t w0[4] = {y0.x, y0.y, y0.z, y0.w}, w1[4] = {y1.x, y1.y, y1.z, y1.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t a = w0[j], b = w1[j];
-    acc[j][0] = lo_f(a);
-    acc[j][1] = hi_f(a);
-    acc[j][2] = lo_f(b);
-    acc[j][3] = hi_f(b);
   }
 }
 // A lane's 8 output columns of row r (0, 1), rounded once.
@@ -200,7 +185,15 @@ __device__ __forceinline__ void expand_step(float (&acc)[4][4], const uint4 (&lo
   }
 }
 
-// Tiles of 16 rows (decode). R: padded rank of the pool.
+// Tiles of 16 rows (decode). R: padded rank of the pool. A cluster of C CTAs per tile: each takes 1/C of
+// K and computes its share of h (16 x R) with mma.sync, the shares meet through the cluster's shared
+// memory, and each CTA then takes 1/C of the columns; h never leaves the cluster. A decode tile holds
+// one to a few rows, so what counts is latency and the bytes of A and B (64 rows over 32 adapters, K
+// 3584, N 4608, rank 16: 7.9 MB, 7.2 us, of which the chain of launch, plan, x and A, exchange, B and y is
+// some 6). Operands go straight from global memory into fragments: the order of k within a 32-value
+// step is free as long as both operands agree, so a lane takes 8 consecutive values (16 bytes) of its
+// row, and the columns of four 8-wide tiles are interleaved so that a lane's accumulators are 8
+// consecutive columns of out (16-byte loads of y, 16-byte stores of out).
 template <int R, bool SILU>
 __global__ void __launch_bounds__(kThreads) lora_row16_kernel(const LoraParams p) {
   constexpr int RT = R / 8;           // 8-wide rank tiles
@@ -405,9 +398,13 @@ __device__ __forceinline__ uint8_t* align1k(uint8_t* p) {
 // (gate and up: 64 of each), and the epilogue adds the product in place of y, from where whole
 // 128-byte rows go out. The rows are gathered, so the ring is filled by cp.async, 16 bytes a thread.
 //
-// It is bound by bytes, so what it takes is few instructions per byte and enough of them in flight.
-// With mma.sync fragments (a warp 16 rows x 32 columns) the same ring was bound by instruction issue:
-// 8185 rows, K 4096, N 6144, rank 64: 72 us, against 240 us without a ring.
+// It is bound by bytes, so what it takes is few instructions per byte and enough bytes in flight. 8185
+// rows, K 4096, N 6144, rank up to 64 (268 MB, 42 us at the copy rate): 240 us with mma.sync fragments
+// loaded from global memory, 72 us with the same behind the ring (bound by instruction issue), 61 us
+// this way (4.4 TB/s). 2048 rows, K 3584, N 37888 with the epilogue (254 MB, 39 us): 151, 62, 59 us.
+// A row's share of a unit is what the memory sees: 64-byte pieces gave 3.3 TB/s in the expand, 128
+// bytes 4.3, 256 bytes 4.7; one CTA of 16 warps per SM instead of two of 8 was slower (66 us: its
+// phases do not overlap).
 template <int R>
 struct Shrink128 {
   static constexpr int kStage = 128 * 128 + R * 128;

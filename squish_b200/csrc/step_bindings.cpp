@@ -77,6 +77,15 @@ void step_layout(torch::Tensor ctx, torch::Tensor q, torch::Tensor tables, torch
   p.tile = (int)tile;
   p.token_cap = (int)cap;
   p.tile_cap = (int)tcap;
+  // (blocks read the lengths while others already write the results)
+  auto apart = [&](const torch::Tensor& t, const char* name, int64_t n) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr()), b = reinterpret_cast<uintptr_t>(out.data_ptr());
+    TORCH_CHECK(n == 0 || a >= b + 4 * out.numel() || b >= a + 4 * n, name, " is part of the step layout it makes");
+  };
+  apart(ctx, "ctx_len", B);
+  apart(q, "q_len", B);
+  apart(free_pages, "free_pages", free_pages.numel());
+  apart(tables, "block_tables", B > 0 ? (B - 1) * tables.stride(0) + tables.size(1) : 0);
   // one buffer, its rows in this order, each padded to a multiple of four (ops.step.StepLayout)
   auto pad = [](int64_t n) { return (n + 3) / 4 * 4; };
   int* at = arr<int>(out, "the step layout", I32, dev,
@@ -177,7 +186,7 @@ void lora_plan(torch::Tensor row_slot, int64_t slots, int64_t tm, torch::Tensor 
   const int64_t M = row_slot.numel();
   TORCH_CHECK(slots >= 1 && slots <= sq::kLoraMaxSlots, "1..", str(sq::kLoraMaxSlots), " adapter slots, not ", str(slots));
   TORCH_CHECK(tm == 16 || tm == 128, "tile rows must be 16 or 128");
-  TORCH_CHECK(M <= (1 << 24), "too many rows");
+  TORCH_CHECK(M <= (1 << 22), "at most 2^22 rows, not ", str(M));
   sq::LoraPlanParams p{};
   p.row_slot = arr<int>(row_slot, "row_slots", I32, dev, 0);
   p.M = (int)M;
@@ -202,12 +211,19 @@ const __nv_bfloat16* rows16(const torch::Tensor& t, const char* name, const torc
               name, " rows must have unit column stride and be 16-byte aligned");
   return reinterpret_cast<const __nv_bfloat16*>(t.data_ptr());
 }
+// Do two bf16 matrices share memory? Column ranges of one buffer (rows of the same stride) do not.
 bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
   if (a.numel() == 0 || b.numel() == 0) return false;
   auto end = [](const torch::Tensor& t) {
     return reinterpret_cast<uintptr_t>(t.data_ptr()) + 2 * ((t.size(0) - 1) * t.stride(0) + t.size(1));
   };
-  return reinterpret_cast<uintptr_t>(a.data_ptr()) < end(b) && reinterpret_cast<uintptr_t>(b.data_ptr()) < end(a);
+  if (reinterpret_cast<uintptr_t>(a.data_ptr()) >= end(b) || reinterpret_cast<uintptr_t>(b.data_ptr()) >= end(a))
+    return false;
+  const int64_t ld = a.stride(0);
+  if (ld != b.stride(0) || ld <= 0 || a.size(0) <= 1 || b.size(0) <= 1) return true;
+  const int64_t d = (reinterpret_cast<intptr_t>(a.data_ptr()) - reinterpret_cast<intptr_t>(b.data_ptr())) / 2;
+  const int64_t col = ((d % ld) + ld) % ld;  // first column of a in rows that start at b's
+  return col < b.size(1) || col + a.size(1) > ld;
 }
 
 void lora_add(torch::Tensor x, torch::Tensor a, torch::Tensor b, torch::Tensor rank, torch::Tensor scale,

@@ -9,6 +9,8 @@
 // share of the token, tile and page rows, found by binary search in the prefixes in shared memory.
 // No block needs another's result: the page of a new token comes from the free list, not from the
 // table entry that another block may be writing. So the step is one launch with no grid-wide wait.
+// What bounds it is latency: launch, lengths, scan, search, page, slot (64 sequences: 3.5 us for 3 KB;
+// 1000 sequences, 250000 tokens: 6.8 us for 3.2 MB).
 #include "kernels.h"
 #include "launch.cuh"
 #include "sm100.cuh"

@@ -1,9 +1,11 @@
 """Serving-step operators: the step's layout on the device, low-rank adapters of many requests,
 scored expert routing and sampling from given uniform numbers.
 
-Like the wrappers in :mod:`.kernels`, every call launches on the current CUDA stream, allocates
-nothing when the caller provides the output, and can be captured in a CUDA graph. None of them
-uses shared scratch memory, so calls on several streams do not disturb one another.
+Like the wrappers in :mod:`.kernels`, every call launches on the current CUDA stream and can be
+captured in a CUDA graph; with the output provided none allocates, but :func:`lora_add` with more
+than 512 rows (a scratch of 4 bytes per row and rank) and :func:`lora_linear` with ``silu_mul`` (the
+projection before the activation), from torch's caching allocator. No scratch memory is shared
+between calls, so calls on several streams, and captured graphs, do not disturb one another.
 """
 from __future__ import annotations
 
@@ -74,7 +76,8 @@ def step_layout(ctx_len: torch.Tensor, q_len: torch.Tensor, block_tables: torch.
 
     What does not fit is not written and records SQ_ERR_BOUNDS in the workspace status: tokens past
     the buffers, pages past the row's width or the end of the free list (their tokens get slot -1).
-    A length below 0 or above 2^30 counts as a resting sequence and records it as well."""
+    A length below 0 or above 2^30 counts as a resting sequence and records it as well. The lengths
+    may not be rows of ``out`` itself (copy ``out.kv_len`` to make it the next step's ``ctx_len``)."""
     b = ctx_len.numel()
     if b != out.seqs:
         out._narrow(b)

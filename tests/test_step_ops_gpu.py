@@ -147,6 +147,14 @@ def test_layout_refusals(cuda):
             call(**kw)
     with pytest.raises(ValueError, match="sequences in a layout"):
         call(c=i32([0] * 3, cuda))
+    with pytest.raises(RuntimeError, match="ctx_len is part of the step layout"):
+        call(c=lay.kv_len)
+    with pytest.raises(RuntimeError, match="q_len is part of the step layout"):
+        call(q=lay.positions[:2])
+    call(c=lay.kv_len.clone())
+    none = ops.StepLayout(2, 8, 0, cuda)  # no tiles wanted, no pages left, a table without columns
+    ops.step_layout(good["c"], i32([0, 0], cuda), good["t"][:, :0], good["f"][:0], 4, none)
+    assert none.totals.tolist() == [0, 0, 0] and status(cuda) == 0
 
 
 # ----------------------------------------------------------------------------- routing
@@ -568,8 +576,9 @@ def test_two_streams_at_once(cuda):
         lg = (torch.randn(9, 40000, generator=g) * 2).to(BF).to(cuda)
         rl = torch.randn(500, 128, generator=g).to(cuda)
         pool, _ = make_adapters(cuda, 2, 512, 512, 16, seed=i)
-        plan = ops.lora_plan((torch.arange(300) % 3 - 1).to(torch.int32).to(cuda), 2)
-        x, y = torch.randn(300, 512, generator=g).to(BF).to(cuda), torch.randn(300, 512, generator=g).to(BF).to(cuda)
+        m = (300, 900)[i]  # (both tile sizes)
+        plan = ops.lora_plan((torch.arange(m) % 3 - 1).to(torch.int32).to(cuda), 2)
+        x, y = torch.randn(m, 512, generator=g).to(BF).to(cuda), torch.randn(m, 512, generator=g).to(BF).to(cuda)
         u, t = torch.rand(9, generator=g).to(cuda), torch.full((9,), 0.8, device=cuda)
         work.append((lg, u, t, rl, pool, plan, x, y))
 
@@ -658,6 +667,63 @@ def test_step_in_a_graph_with_new_lengths(cuda):
             assert st["tok"].tolist() == [sample_ref(host[b], u[b], 1.0)[0] for b in range(B)]
             assert np.array_equal(st["ids"].view(cap, 4).cpu().numpy(), want_ids)
     assert status(cuda) == 0
+
+
+@pytest.mark.parametrize("m", [40, 700])
+@pytest.mark.parametrize("silu", [False, True])
+def test_lora_in_two_graphs(cuda, m, silu):
+    """Two captured graphs of one plan and pool, replayed in turn and next to eager calls, with new rows
+    and a new adapter between replays."""
+    k, n = 264, 256
+    g = torch.Generator().manual_seed(m)
+    pool, ads = make_adapters(cuda, 3, k, n, 16)
+    slot = torch.full((m,), -1, dtype=torch.int32, device=cuda)
+    plan = ops.LoraPlan(m, 3, cuda)
+    pairs = []
+    for _ in range(2):
+        x, y = torch.randn(m, k, generator=g).to(BF).to(cuda), torch.randn(m, n, generator=g).to(BF).to(cuda)
+        out = torch.zeros(m, n // 2 if silu else n, dtype=BF, device=cuda)
+        ops.lora_plan(slot, 3, out=plan)
+        ops.lora_add(x, pool, plan, y, out=out, silu_mul=silu)  # warm up
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            ops.lora_plan(slot, 3, out=plan)
+            ops.lora_add(x, pool, plan, y, out=out, silu_mul=silu)
+        pairs.append((gr, x, y, out))
+    for it in range(3):
+        rows = torch.randint(-1, 3, (m,), generator=g)
+        slot.copy_(rows)
+        a, b = (torch.randn(5, k, generator=g) / 16).to(BF), (torch.randn(n, 5, generator=g) * 0.3).to(BF)
+        pool.load(it, a, b, 1.5)
+        ads[it] = (a, b, 1.5)
+        for gr, *_ in pairs:
+            gr.replay()
+        for _, x, y, out in pairs:
+            want, tol = lora_ref(x, y, rows, ads, silu)
+            assert ((out.double().cpu() - want).abs() <= tol).all()
+            eager = ops.lora_add(x, pool, ops.lora_plan(slot, 3), y, silu_mul=silu)
+            assert torch.equal(eager, out)
+    assert status(cuda) == 0
+
+
+def test_lora_column_ranges_of_one_buffer(cuda):
+    """x, y and out as column ranges of the same rows."""
+    m, k, n = 33, 64, 128
+    pool, ads = make_adapters(cuda, 2, k, n, 8)
+    rows = torch.arange(m) % 3 - 1
+    plan = ops.lora_plan(rows.to(torch.int32).to(cuda), 2)
+    buf = torch.randn(m, 400, generator=torch.Generator().manual_seed(0)).to(BF).to(cuda)
+    keep = buf.clone()
+    x, y, out = buf[:, 8:72], buf[:, 72:200], buf[:, 200:328]
+    ops.lora_add(x, pool, plan, y, out=out)
+    want, tol = lora_ref(keep[:, 8:72], keep[:, 72:200], rows, ads)
+    assert ((out.double().cpu() - want).abs() <= tol).all()
+    assert torch.equal(buf[:, :200], keep[:, :200]) and torch.equal(buf[:, 328:], keep[:, 328:])
+    ops.lora_add(x, pool, plan, y, out=y)  # in place, next to its input
+    assert torch.equal(y, out)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ops.lora_add(x, pool, plan, y, out=buf[:, 64:192])
 
 
 @pytest.mark.parametrize("pad_tiles", [0, 7])
