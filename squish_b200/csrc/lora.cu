@@ -145,6 +145,7 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
   return g * r * u;
 }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 // y added to the accumulators of 16 rows x 32 columns: a lane's 8 columns of its two rows.
 __device__ __forceinline__ void add_to(float (&acc)[4][4], uint4 y0, uint4 y1) {
   const uint32_t w0[4] = {y0.x, y0.y, y0.z, y0.w}, w1[4] = {y1.x, y1.y, y1.z, y1.w};
@@ -203,24 +204,39 @@ __global__ void __launch_bounds__(kThreads) lora_row16_kernel(const LoraParams p
   constexpr int HS = R + 8;           // row stride of the bf16 parts of h
   pdl_wait();
   pdl_trigger();
-  if ((int)blockIdx.x >= *p.num_tiles) return;  // the whole cluster
+  // (loads that need not wait for one another are issued together: a decode tile is a chain of waits)
+  const int nt = *p.num_tiles;
   const int4 tile = p.tiles[blockIdx.x];
+  if ((int)blockIdx.x >= nt) return;  // the whole cluster
   const int slot = tile.x, cnt = tile.z;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int row0 = g < cnt ? p.order[tile.y + g] : -1, row1 = g + 8 < cnt ? p.order[tile.y + g + 8] : -1;
+  const int fetch = (tid >> 4) < cnt ? p.order[tile.y + (tid >> 4)] : -1;
   const int rank = slot >= 0 ? p.rank[slot] : 0;
+  const float sc = slot >= 0 ? p.scale[slot] : 0.f;
   if (rank <= 0 && p.in_place) return;
   extern __shared__ __align__(16) uint8_t smem[];
   float* part = reinterpret_cast<float*>(smem);                                    // [KW][ROWS][PS]
   __nv_bfloat16* hh = reinterpret_cast<__nv_bfloat16*>(part + KW * ROWS * PS);     // [2][ROWS][HS]
-  __shared__ int rows[ROWS];
   cg::cluster_group cl = cg::this_cluster();
   const int C = gridDim.z, cr = blockIdx.z;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g = lane >> 2, t = lane & 3;
   const int kw = warp;
-  if (tid < ROWS) rows[tid] = tid < cnt ? p.order[tile.y + tid] : -1;
-  __syncthreads();
-  const int row0 = rows[g], row1 = rows[g + 8];
-  const int live = min(R, (rank + 15) / 16 * 16);  // ranks computed: whole 16-wide steps
+  const int live = R == 16 ? 16 : min(R, (rank + 15) / 16 * 16);  // ranks computed: whole 16-wide steps
+
+  // this CTA's columns, in units of 32 output columns; its part of B (consecutive rows) and of y goes on
+  // its way to L2 while h is computed
+  constexpr int G = SILU ? 2 : 1;  // column groups of a unit (gate and up)
+  const int units = SILU ? p.N / 64 : (p.N + 31) / 32;
+  const int u0 = (int)((long long)units * cr / C), u1 = (int)((long long)units * (cr + 1) / C);
+  const __nv_bfloat16* bs = p.b + (size_t)(slot < 0 ? 0 : slot) * p.N * R;
+  {
+    const int n0 = u0 * 32 * G, n1 = min(p.N, u1 * 32 * G);
+    if (rank > 0)
+      for (size_t e = (size_t)n0 * R + tid * 64; e < (size_t)n1 * R; e += kThreads * 64) prefetch_l2(bs + e);
+    if (fetch >= 0)
+      for (int c = n0 + (tid & 15) * 64; c < n1; c += 16 * 64) prefetch_l2(p.y + fetch * p.ldy + c);
+  }
 
   if (rank > 0) {
     // ---- h share: this warp's 32-wide steps of K
@@ -281,7 +297,6 @@ __global__ void __launch_bounds__(kThreads) lora_row16_kernel(const LoraParams p
     }
     cl.sync();
     // ---- h of the tile: sum of the CTAs' shares, in rank order; scaled, split into two bf16
-    const float sc = p.scale[slot];
     for (int i = tid; i < ROWS * nv; i += kThreads) {
       const int r = i / nv, c = (i % nv) * 4;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -301,12 +316,12 @@ __global__ void __launch_bounds__(kThreads) lora_row16_kernel(const LoraParams p
       *reinterpret_cast<uint2*>(hh + (ROWS + r) * HS + c) =
           make_uint2(pack_bf16(s.x - lo_f(h01), s.y - hi_f(h01)), pack_bf16(s.z - lo_f(h23), s.w - hi_f(h23)));
     }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (waited for at the end)
     __syncthreads();
   }
 
-  // ---- out = y + h B^T over this CTA's columns, 32 output columns per step
+  // ---- out = y + h B^T over this CTA's columns
   constexpr int KS = R == 16 ? 1 : R / 32;  // rank steps (32 wide; one of 16 for R = 16)
-  constexpr int G = SILU ? 2 : 1;           // column groups of a step (gate and up)
   uint4 fa[2][KS][2];                       // [upper / lower][step][row g / g + 8]
   if (rank > 0) {
 #pragma unroll
@@ -326,9 +341,6 @@ __global__ void __launch_bounds__(kThreads) lora_row16_kernel(const LoraParams p
           }
         }
   }
-  const __nv_bfloat16* bs = p.b + (size_t)(slot < 0 ? 0 : slot) * p.N * R;
-  const int units = SILU ? p.N / 64 : (p.N + 31) / 32;
-  const int u0 = (int)((long long)units * cr / C), u1 = (int)((long long)units * (cr + 1) / C);
   for (int u = u0 + kw; u < u1; u += KW) {
     float acc[G][4][4];
     uint4 yv[G][2];  // loaded first, added last: the products do not wait for it
@@ -372,7 +384,8 @@ __global__ void __launch_bounds__(kThreads) lora_row16_kernel(const LoraParams p
       if (row1 >= 0) *reinterpret_cast<uint4*>(p.out + row1 * p.ldo + oc) = finish<SILU, G>(acc, 1);
     }
   }
-  if (rank > 0) cl.sync();  // peers may still read this CTA's share
+  // peers may have read this CTA's share until now
+  if (rank > 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- tiles of 128 rows (prefill)
