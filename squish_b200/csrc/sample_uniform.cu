@@ -705,8 +705,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_uniform_kernel(const Sampl
   // ---- the non-empty bins of this CTA's share (1/C of the signed values; zero goes with the smallest
   // positive ones), as a list in descending order of value, so that afterwards the exponentials (a few
   // hundred cycles each) spread evenly over the threads. A warp takes 1/16 of the share, its lanes
-  // neighbouring bins: a ballot per 32 bins, first to count, then to place.
-  constexpr int kChunks = kShare / (32 * kWarps);
+  // neighbouring bins, 16 bytes of counters at a time, first to count, then to place.
+  constexpr int kChunks = kShare / (128 * kWarps);
   unsigned short* list = reinterpret_cast<unsigned short*>(own + (C > 1 ? kShare + 4 : 0));
   auto count = [&](int j) -> int {
     const int a = main_at(bin_bits(j, -1));
@@ -715,19 +715,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_uniform_kernel(const Sampl
   };
   int len;
   {
-    const int i0 = (rank * kWarps + (tid >> 5)) * kChunks * 32;
-    const bool with_zero = i0 + kChunks * 32 == kMagN && count(kMagN) > 0;
+    const int i0 = (rank * kWarps + (tid >> 5)) * kChunks * 128;
+    const bool with_zero = i0 + kChunks * 128 == kMagN && count(kMagN) > 0;
+    // the warp's counters are consecutive (downwards for positive values, upwards for negative ones): a
+    // lane takes four neighbours at a time; flags: bit 4 k + b = its b-th bin of chunk k is not empty
+    const bool up = i0 >= kMagN;
+    const int* c0 = (C > 1 ? own - block : hist) + main_at(bin_bits(nth_bin(i0), -1)) + (up ? 4 * lane : -4 * lane - 3);
     unsigned flags = 0;
-    int filled = with_zero;
-    // (the warp's counters are consecutive: downwards for positive values, upwards for negative ones)
-    const int dir = i0 < kMagN ? -1 : 1;
-    const int* c0 = (C > 1 ? own - block : hist) + main_at(bin_bits(nth_bin(i0), -1)) + dir * lane;
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-      const bool f = c0[dir * 32 * k] > 0;
-      flags |= (f ? 1u : 0u) << k;
-      filled += __popc(__ballot_sync(0xffffffffu, f));
+      const int4 v = *reinterpret_cast<const int4*>(c0 + (up ? 128 * k : -128 * k));
+      const unsigned f = (v.x > 0 ? 1u : 0u) | (v.y > 0 ? 2u : 0u) | (v.z > 0 ? 4u : 0u) | (v.w > 0 ? 8u : 0u);
+      flags |= (up ? f : __brev(f) >> 28) << (4 * k);
     }
+    const int filled = __reduce_add_sync(0xffffffffu, __popc(flags)) + with_zero;
     if (lane == 0) sh.cnt[tid >> 5] = filled;
     __syncthreads();
     int at = 0;
@@ -739,12 +740,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_uniform_kernel(const Sampl
     }
     if (filled > 0) {
       const unsigned below = (1u << lane) - 1u;
-      const int j0 = nth_bin(i0) + lane;
+      const int j0 = nth_bin(i0) + 4 * lane;
 #pragma unroll
       for (int k = 0; k < kChunks; ++k) {
-        const unsigned m = __ballot_sync(0xffffffffu, (flags >> k) & 1u);
-        if ((flags >> k) & 1u) list[at + __popc(m & below)] = (unsigned short)(j0 + 32 * k);
-        at += __popc(m);
+        const unsigned f = (flags >> (4 * k)) & 15u;
+        unsigned m[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) m[b] = __ballot_sync(0xffffffffu, (f >> b) & 1u);
+        if ((m[0] | m[1] | m[2] | m[3]) == 0u) continue;
+        int to = at, next = at;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          to += __popc(m[b] & below);
+          next += __popc(m[b]);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if ((f >> b) & 1u) list[to++] = (unsigned short)(j0 + 128 * k + b);
+        at = next;
       }
       if (with_zero && lane == 0) list[at] = (unsigned short)kMagN;
     }
