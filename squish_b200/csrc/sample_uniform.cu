@@ -24,8 +24,8 @@
 // bins (summed over the peers' shared memory); three exchanges through shared memory (masses, kept
 // masses, the drawn value) make the draw, and a fourth keeps the memory alive.
 //
-// Measured (V 152064, temperature only): 1 row 15 us (a chain of five cluster exchanges and as many
-// block sums in fp64, 28000 clocks), 64 rows 25 us, 256 rows 52 us (78 MB: 12 us at the copy rate; 15 us a
+// Measured (V 152064, temperature only): 1 row 16 us (a chain of five cluster exchanges and as many
+// block sums in fp64, 27000 clocks), 64 rows 23 us, 256 rows 52 us (78 MB: 12 us at the copy rate; 15 us a
 // row on its SM are the atomics, at 2.8 clocks per warp). With one exponential per token, serial walks
 // over a thread's bins and counters read in the owner's order it was 34, 78 and 122 us.
 #include <cooperative_groups.h>
@@ -912,14 +912,17 @@ cudaError_t launch_c(const SampleUniformParams& p, cudaStream_t s) {
 cudaError_t sample_uniform_launch(const SampleUniformParams& p, int num_sms, cudaStream_t s) {
   if (p.B == 0) return cudaSuccess;
   if (p.V <= 0) return cudaErrorInvalidValue;
-  // CTAs per row: as many as the SMs hold at one row each, at least 4096 values per CTA
-  // (two do not pay: their histogram, sums and list leave room for one CTA per SM)
-  int c = 8;
-  if ((long long)p.B * c > 2 * num_sms || p.V / c < 4096) c = 4;
-  if ((long long)p.B * c > 2 * num_sms || p.V / c < 4096) c = 1;
+  // CTAs per row. A cluster counts its row faster and pays for it with exchanges: up to 32000 values one
+  // CTA is as fast or faster at any batch (1 row of 32000: 13.2 us against 13.9, 13.1, 13.9 with 2, 4, 8;
+  // 64 rows: 13.7 against 14.3, 20.3, 42.2). Of 152064 values, us with 1, 2, 4, 8 CTAs: 1 row 23, 19, 17,
+  // 16; 8 rows 30, 23, 19, 17; 16 rows 30, 23, 18, 20; 64 rows 30, 23, 26, 47; 100 rows 31, 42, 43, 75 (two
+  // CTAs of two do not fit an SM).
+  int c = 1;
+  if (p.V > 65536) c = 16 * p.B <= num_sms ? 8 : 8 * p.B <= num_sms ? 4 : 2 * p.B <= num_sms ? 2 : 1;
   switch (c) {
     case 8: return launch_c<8>(p, s);
     case 4: return launch_c<4>(p, s);
+    case 2: return launch_c<2>(p, s);
     default: return launch_c<1>(p, s);
   }
 }

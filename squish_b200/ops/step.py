@@ -216,7 +216,10 @@ class LoraPlan:
 
     def __init__(self, rows: int, slots: int, device):
         # tiles of 16 rows while adapters have few rows each, of 128 for prefill: a tile reads its
-        # adapter once, so wider tiles re-read less (from L2) but leave more of themselves empty
+        # adapter once, so wider tiles re-read less (from L2) but leave more of themselves empty.
+        # Measured on a B200 with 16 / 128, us: 3584 x 3584 rank 16, 16 adapters: 512 rows 9.8 / 12.5,
+        # 1024 rows 12.4 / 13.4; 4096 x 6144 rank 64, 16 adapters: 512 rows 19.4 / 23.3, 1024 rows
+        # 24.7 / 23.8, one adapter: 256 rows 14.4 / 11.1, 512 rows 20.0 / 12.5, 1024 rows 36.6 / 17.1
         self.tile_rows = 16 if rows <= 512 else 128
         self.rows, self.slots = rows, slots
         self.max_tiles = -(-rows // self.tile_rows) + min(slots + 1, rows)
