@@ -66,10 +66,13 @@ struct Shared {
     int first, cnt;  // first non-empty bin of the CTA's range, tokens
   } in[8];
   double scale[8];  // their masses on the row's scale
-  int edge;         // thread at the end of the kept prefix, -1
-  int e_first, e_n; // its entries, and what precedes them
-  long long e_n0;
-  double e_m0;
+  int edge;  // thread at the end of the kept prefix (kThreads: none)
+  // its entries and what precedes them
+  struct {
+    int first, n;
+    long long n0;
+    double m0;
+  } end;
   int r_bits, r_rank;
 };
 
@@ -620,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_uniform_kernel(const Sampl
   for (int i = tid; i < kHist / 4; i += kThreads) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
   if (tid == 0) {
     sh.odd = 0;
-    sh.edge = -1;
+    sh.edge = kThreads;
   }
   __syncthreads();
   {
@@ -836,17 +839,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_uniform_kernel(const Sampl
   // prefix, a part (every warp works that part out)
   const bool any = n > 0 && (n0 == 0 || (n0 < rule.K && m0 < rule.border && w_hi >= rule.min_p));
   const bool whole = any && n0 + n <= rule.K && m0 + mass < rule.border && w_lo >= rule.min_p;
-  if (any && !whole) {
-    sh.edge = tid;
-    sh.e_first = e0;
-    sh.e_n = e1 - e0;
-    sh.e_n0 = n0;
-    sh.e_m0 = m0;
-  }
+  // (rounding may let a later thread think that it is the one: the first counts)
+  if (any && !whole) atomicMin(&sh.edge, tid);
   double cta_kept = block_sum(sh, 0, whole ? mass : 0.0);
   const int edge = sh.edge;
-  if (edge >= 0)
-    cta_kept += warp_walk(rule, bin, count, sh.e_first, sh.e_n, sh.e_m0, sh.e_n0, -1.0, nullptr, nullptr);
+  if (edge < kThreads) {
+    if (tid == edge) sh.end = {e0, e1 - e0, n0, m0};
+    __syncthreads();
+    cta_kept += warp_walk(rule, bin, count, sh.end.first, sh.end.n, sh.end.m0, sh.end.n0, -1.0, nullptr, nullptr);
+  }
   double total = cta_kept;
   int sel = 0;  // CTA that holds the target
   if constexpr (C > 1) {

@@ -368,6 +368,39 @@ def test_sample_unusual_values(cuda, C_rows):
         run_sample(cuda, logits, u, temps, top_p, top_k, min_p)
 
 
+@pytest.mark.parametrize("V", [9000, 70001])
+def test_sample_masked_unusual_values(cuda, V):
+    """Infinities, NaN and values outside the main bins in masked places do not count."""
+    g = torch.Generator().manual_seed(1)
+    B = 6
+    logits = torch.randn(B, V, generator=g) * 2
+    mask = torch.rand(B, V, generator=g) < 0.7
+    mask[:, 17] = True
+    bad = torch.tensor([math.inf, math.nan, 1e20, -math.inf, 1e-20, -1e-30])
+    for b in range(B):
+        where = torch.nonzero(~mask[b]).flatten()[::5]
+        logits[b, where] = bad[torch.arange(len(where)) % len(bad)]
+    rng = random.Random(3)
+    lg = logits.to(BF).to(cuda)
+    run_sample(cuda, lg, *rand_params(rng, B), mask=mask)
+    run_sample(cuda, lg, [rng.random() for _ in range(B)], [1.0] * B, mask=mask)
+    run_sample(cuda, lg, [0.5] * B, [0.0] * B, mask=mask)
+
+
+@pytest.mark.parametrize("B,V", [(1, 65537), (9, 70000), (18, 66001), (40, 80003), (74, 65600), (75, 65600)])
+def test_sample_rows_shared_by_ctas(cuda, B, V):
+    """Each number of CTAs per row, at its borders, with some rows greedy and some without a token."""
+    g = torch.Generator().manual_seed(V)
+    rng = random.Random(B)
+    logits = (torch.randn(B, V, generator=g) * 3).to(BF)
+    if B > 1:
+        logits[B // 2] = -math.inf
+        logits[B - 1] = 0.0
+        logits[0, 1234] = 1e-12  # outside the main bins: one CTA does the row
+    u, temp, top_p, top_k, min_p = rand_params(rng, B)
+    run_sample(cuda, logits.to(cuda), u, temp, top_p, top_k, min_p)
+
+
 def test_sample_strides_and_optional_parameters(cuda):
     g = torch.Generator().manual_seed(2)
     big = (torch.randn(7, 5003, generator=g) * 2).to(BF).to(cuda)
