@@ -149,7 +149,7 @@ __device__ __forceinline__ int short_list(const uint32_t (&k)[EPL], int K, float
   }
   if (bound != 0u && margin > 0.f) {
     const float v = unord32(bound);
-    bound = v > kNegInf ? ord32(v - margin * (1.f + fabsf(v))) : 1u;
+    if (v < INFINITY) bound = v > kNegInf ? ord32(v - margin * (1.f + fabsf(v))) : 1u;
   }
   bound = max(bound, 1u);  // (fewer open lanes than picks: every open value)
   int n = 0;
@@ -472,6 +472,10 @@ __global__ void __launch_bounds__(kWarps * 32) route_scored_kernel(const RouteSc
     if (on) {
       const float ex = expf(-fabsf(xi));
       s = si >= 0.f ? si : (xi >= 0.f ? 1.f : ex) / (1.f + ex);
+    }
+    if (p.renorm) {  // far below 0 a sigmoid is the exponential: relative to the largest it does not underflow
+      const float mm = unord32(__reduce_max_sync(kFull, ord32(xi)));
+      if (mm < -30.f) s = xi > kNegInf ? expf(xi - mm) : 0.f;
     }
   } else {
     // renormalised: relative to the largest pick, the softmax denominator cancels (next to an

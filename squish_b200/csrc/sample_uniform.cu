@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_uniform_kernel(const Sampl
       }
     }
     float top = fmaxf(__low2float(best), __high2float(best));
-    top = top == top ? top : -INFINITY;
+    top = top == 0.f ? 0.f : top == top ? top : -INFINITY;  // (zeros of both signs are one value: one key)
     const unsigned tb = __float_as_uint(top);
     // bf16 keys are the upper halves of fp32 keys: a minimum of complements is a maximum
     int key = -(int)(((tb & 0x80000000u) ? ~tb : (tb | 0x80000000u)) >> 16);

@@ -251,6 +251,31 @@ def test_route_infinities_and_nan(cuda, score, groups):
                   group_score="top2")
 
 
+@pytest.mark.parametrize("k", [4, 20])
+def test_route_infinite_bias(cuda, k):
+    """A bias of +inf puts experts first, of -inf last, however many."""
+    g = torch.Generator().manual_seed(8)
+    logits = torch.randn(6, 64, generator=g).to(cuda)
+    for n in (1, k, 30):
+        bias = torch.randn(64, generator=g) * 0.1
+        bias[torch.randperm(64, generator=g)[:n]] = math.inf
+        bias[torch.randperm(64, generator=g)[:3]] = -math.inf
+        for kw in (dict(), dict(groups=8, top_groups=4), dict(groups=8, top_groups=4, group_score="top2")):
+            run_route(cuda, logits, k, bias=bias.to(cuda), score="sigmoid", **kw)
+            run_route(cuda, logits, k, bias=bias.to(cuda), score="softmax", **kw)
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("shift", [-25.0, -35.0, -100.0, -300.0])
+def test_route_small_sigmoids_are_renormalised(cuda, shift, bias):
+    """Scores below what fp32 holds still give weights that sum to 1."""
+    g = torch.Generator().manual_seed(9)
+    logits = (torch.randn(6, 64, generator=g) * 2 + shift).to(cuda)
+    logits[1, 5:] = -math.inf
+    b = (torch.randn(64, generator=g) * 0.1).to(cuda) if bias else None
+    run_route(cuda, logits, 8, bias=b, score="sigmoid")
+
+
 def test_route_strides(cuda):
     g = torch.Generator().manual_seed(3)
     big = torch.randn(9, 300, generator=g).to(BF).to(cuda)
@@ -399,6 +424,19 @@ def test_sample_rows_shared_by_ctas(cuda, B, V):
         logits[0, 1234] = 1e-12  # outside the main bins: one CTA does the row
     u, temp, top_p, top_k, min_p = rand_params(rng, B)
     run_sample(cuda, logits.to(cuda), u, temp, top_p, top_k, min_p)
+
+
+@pytest.mark.parametrize("B", [2, 12, 30, 80])
+def test_sample_greedy_zeros_of_both_signs(cuda, B):
+    """-0 and +0 are equal: the lower index wins, whichever CTA of the row holds it."""
+    V = 70001
+    logits = torch.full((B, V), -1.0)
+    logits[:, 11] = -0.0
+    logits[:, V - 2] = 0.0
+    logits[1, 11], logits[1, V - 2] = 0.0, -0.0
+    tok = torch.empty(B, dtype=torch.int32, device=cuda)
+    ops.sample_uniform(logits.to(BF).to(cuda), torch.full((B,), 0.5, device=cuda), tok)
+    assert tok.tolist() == [11] * B
 
 
 def test_sample_strides_and_optional_parameters(cuda):
