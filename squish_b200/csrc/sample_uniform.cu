@@ -67,12 +67,12 @@ struct Shared {
   } in[8];
   double scale[8];  // their masses on the row's scale
   int edge;  // thread at the end of the kept prefix (kThreads: none)
-  // its entries and what precedes them
+  // its entries and what precedes them, per warp
   struct {
     int first, n;
     long long n0;
     double m0;
-  } end;
+  } end[kWarps];
   int r_bits, r_rank;
 };
 
@@ -840,13 +840,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_uniform_kernel(const Sampl
   const bool any = n > 0 && (n0 == 0 || (n0 < rule.K && m0 < rule.border && w_hi >= rule.min_p));
   const bool whole = any && n0 + n <= rule.K && m0 + mass < rule.border && w_lo >= rule.min_p;
   // (rounding may let a later thread think that it is the one: the first counts)
-  if (any && !whole) atomicMin(&sh.edge, tid);
+  const unsigned ends = __ballot_sync(0xffffffffu, any && !whole);
+  if (ends != 0 && lane == __ffs(ends) - 1) {
+    atomicMin(&sh.edge, tid);
+    sh.end[tid >> 5] = {e0, e1 - e0, n0, m0};
+  }
   double cta_kept = block_sum(sh, 0, whole ? mass : 0.0);
   const int edge = sh.edge;
   if (edge < kThreads) {
-    if (tid == edge) sh.end = {e0, e1 - e0, n0, m0};
-    __syncthreads();
-    cta_kept += warp_walk(rule, bin, count, sh.end.first, sh.end.n, sh.end.m0, sh.end.n0, -1.0, nullptr, nullptr);
+    const auto& end = sh.end[edge >> 5];
+    cta_kept += warp_walk(rule, bin, count, end.first, end.n, end.m0, end.n0, -1.0, nullptr, nullptr);
   }
   double total = cta_kept;
   int sel = 0;  // CTA that holds the target

@@ -44,6 +44,8 @@ class StepLayout:
                  tile: int = LAYOUT_TILE):
         if max_seqs < 1 or max_tokens < 1:
             raise ValueError("a step layout holds at least one sequence and one token")
+        if tile < 1:
+            raise ValueError("an attention tile has at least one query")
         if max_tiles is None:
             max_tiles = max_tokens // tile + min(max_seqs, max_tokens)
         self.max_seqs, self.max_tokens, self.max_tiles, self.tile = max_seqs, max_tokens, max_tiles, tile
@@ -76,7 +78,7 @@ def step_layout(ctx_len: torch.Tensor, q_len: torch.Tensor, block_tables: torch.
 
     What does not fit is not written and records SQ_ERR_BOUNDS in the workspace status: tokens past
     the buffers, pages past the row's width or the end of the free list (their tokens get slot -1).
-    A length below 0 or above 2^30 counts as a resting sequence and records it as well. The lengths
+    A sequence with a length below 0 or of 2^30 tokens and more counts as resting and records it as well. The lengths
     may not be rows of ``out`` itself (copy ``out.kv_len`` to make it the next step's ``ctx_len``)."""
     b = ctx_len.numel()
     if b != out.seqs:
@@ -249,7 +251,9 @@ def lora_add(x: torch.Tensor, pool: LoraPool, plan: LoraPlan, y: torch.Tensor, o
              silu_mul: bool = False, ws: Workspace | None = None) -> torch.Tensor:
     """out[t] = y[t] + scale_s B_s (A_s x[t]) for row t with adapter slot s, out[t] = y[t] without
     one; x [M, K], y [M, N] bf16. ``out`` may be y itself. With ``silu_mul`` the columns of y are
-    interleaved gate/up blocks of 64 and out = silu(gate) * up has N/2 columns."""
+    interleaved gate/up blocks of 64 and out = silu(gate) * up has N/2 columns. Sums are fp32, ``out``
+    is rounded once. Where A_s x[t] is not finite the row may hold NaN for an infinity; other rows do
+    not notice."""
     if out is None:
         out = torch.empty((x.shape[0], pool.n // 2 if silu_mul else pool.n), dtype=torch.bfloat16, device=x.device)
     native().lora_add(x, pool.a, pool.b, pool.rank, pool.scale, y, out, plan.order, plan.tiles, plan.num_tiles,
@@ -261,7 +265,8 @@ def lora_add(x: torch.Tensor, pool: LoraPool, plan: LoraPlan, y: torch.Tensor, o
 def lora_linear(x: torch.Tensor, w: Int4Weight, pool: LoraPool, plan: LoraPlan, out: torch.Tensor | None = None,
                 residual: torch.Tensor | None = None, silu_mul: bool = False,
                 ws: Workspace | None = None) -> torch.Tensor:
-    """:func:`w4a16_linear` with the rows' adapters added (before the SiLU*up epilogue)."""
+    """:func:`w4a16_linear` with the rows' adapters added (before the SiLU*up epilogue). The projection
+    (with the residual) is rounded to bf16 before the adapters are added, and their sum again."""
     if not silu_mul:
         y = w4a16_linear(x, w, out=out, residual=residual, ws=ws)
         return lora_add(x, pool, plan, y, out=y, ws=ws)

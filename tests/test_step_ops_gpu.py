@@ -426,6 +426,18 @@ def test_sample_rows_shared_by_ctas(cuda, B, V):
     run_sample(cuda, logits.to(cuda), u, temp, top_p, top_k, min_p)
 
 
+@pytest.mark.parametrize("V", [1, 4099, 70001])
+def test_sample_extreme_parameters(cuda, V):
+    """The ends of each parameter's range, and what lies behind them."""
+    cases = [(t, p, k, m) for t in (1e-40, 1e-6, 1e30, math.inf)
+             for p, k, m in ((1.0, 0, 0.0), (0.0, 0, 0.0), (-1.0, 0, 0.0), (2.0, 2**31 - 1, -1.0), (0.5, -5, 0.0),
+                             (1.0, 0, 1.0), (1.0, 0, 2.0), (1e-30, 7, 1e-30), (1.0 - 2.0**-24, 0, 0.0))]
+    B = len(cases)
+    logits = (torch.randn(B, V, generator=torch.Generator().manual_seed(V)) * 2).to(BF).to(cuda)
+    for u in (0.0, 2.0**-24, 0.37, 1.0 - 2.0**-24):
+        run_sample(cuda, logits, [u] * B, *map(list, zip(*cases)))
+
+
 @pytest.mark.parametrize("B", [2, 12, 30, 80])
 def test_sample_greedy_zeros_of_both_signs(cuda, B):
     """-0 and +0 are equal: the lower index wins, whichever CTA of the row holds it."""
