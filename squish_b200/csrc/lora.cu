@@ -594,12 +594,15 @@ struct Expand128 {
   static constexpr int S = kFit > 4 ? 4 : kFit;
   static constexpr int kSmem = kA + S * kStage + 1024;
   static constexpr int kCols = G * 64;
+  static constexpr int T = kCtas == 2 ? 256 : 512;  // threads
 };
 
 template <int R, bool SILU>
-__global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expand128_kernel(const LoraParams p) {
+__global__ void __launch_bounds__((Expand128<R, SILU>::T), (Expand128<R, SILU>::kCtas))
+lora_expand128_kernel(const LoraParams p) {
   using TC = Expand128<R, SILU>;
-  constexpr int S = TC::S, G = TC::G;
+  constexpr int S = TC::S, G = TC::G, T = TC::T;
+  constexpr int RP = T / 8, RJ = 128 / RP;  // rows per pass of the block's copies, passes
   constexpr int OQ = SILU ? 1 : G;  // 64-column halves of the output of a unit
   static_assert(S >= 2 && TC::kStage % 1024 == 0, "ring");
   // The launch before this one is the shrink, which lets this one start once everything before it is
@@ -636,20 +639,20 @@ __global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expa
   const int units = (p.N + 64 * G - 1) / (64 * G);
   const int u0 = blockIdx.x * p.units, n2 = min(p.units, units - u0);
 
-  // a thread copies chunk tid % 8 of rows tid / 8 + 32 j of y (and of out), and pieces of B rows
+  // a thread copies chunk tid % 8 of rows tid / 8 + RP j of y (and of out), and pieces of B rows
   const int lr = tid >> 3, lc = tid & 7;
-  const __nv_bfloat16* py[4];
-  __nv_bfloat16* po[4];
+  const __nv_bfloat16* py[RJ];
+  __nv_bfloat16* po[RJ];
   unsigned on = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = rows[lr + 32 * j];
+  for (int j = 0; j < RJ; ++j) {
+    const int r = rows[lr + RP * j];
     on |= (r >= 0 ? 1u : 0u) << j;
     py[j] = p.y + (r < 0 ? 0 : r) * p.ldy + (long long)u0 * 64 * G + lc * 8;
     po[j] = p.out + (r < 0 ? 0 : r) * p.ldo + (long long)u0 * 64 * OQ + lc * 8;
   }
   constexpr int CH = R / 8;          // 16-byte pieces of a B row
-  constexpr int BN = kThreads / CH;  // B rows per pass
+  constexpr int BN = T / CH;         // B rows per pass
   const int bn = tid / CH, bc = tid % CH;
   const __nv_bfloat16* pb = p.b + ((size_t)(slot < 0 ? 0 : slot) * p.N + (size_t)u0 * 64 * G + bn) * R + bc * 8;
   const int so = sw(lr, lc);
@@ -659,11 +662,11 @@ __global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expa
     wr = wr == S - 1 ? 0 : wr + 1;
     if (i < n2) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < RJ; ++j) {
 #pragma unroll
         for (int q = 0; q < G; ++q) {
           const bool in = SILU || col + q * 64 + lc * 8 < p.N;
-          cp16(st + q * 16384 + so + j * 4096, in ? py[j] + q * 64 : p.y, in && ((on >> j) & 1u));
+          cp16(st + q * 16384 + so + j * RP * 128, in ? py[j] + q * 64 : p.y, in && ((on >> j) & 1u));
         }
         py[j] += 64 * G;
       }
@@ -687,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expa
   pdl_wait();
   pdl_trigger();
   if (live > 0) {  // h of the tile, as the A operand
-    for (int e = tid; e < 128 * 2 * CH; e += kThreads) {
+    for (int e = tid; e < 128 * 2 * CH; e += T) {
       const int r = e / (2 * CH), q = e / CH % 2, c = e % CH;
       if (c * 8 < live) {
         const int at = R >= 64 ? (q * (R / 64) + (c >> 3)) * 16384 + sw(r, c & 7) : sw(r, q * CH + c);
@@ -696,7 +699,8 @@ __global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expa
     }
   }
   cp_commit();
-  const int row = (warp & 3) * 32 + lane, hf = warp >> 2;  // this thread's row and half of the columns
+  constexpr int TQ = 8192 / T;                             // columns of a half per thread
+  const int row = (warp & 3) * 32 + lane, hf = warp >> 2;  // this thread's row and part of the columns
   const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
   constexpr uint32_t idesc = idesc_bf16_f32(128, TC::kPair ? 64 : 64 * G);
   int rd = 0;
@@ -729,12 +733,12 @@ __global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expa
       mbar_wait(&done, (uint32_t)i & 1u, p.status, SQ_ERR_TIMEOUT_ACC);
       tc_fence_after();
     }
-    // 32 output columns of each half of the thread's row, 16 at a time, in place of y
+    // the thread's output columns of each half of its row, 16 at a time, in place of y
 #pragma unroll
     for (int oq = 0; oq < OQ; ++oq) {
 #pragma unroll
-      for (int c = 0; c < 32; c += 16) {
-        const int c0 = hf * 32 + c;
+      for (int c = 0; c < TQ; c += 16) {
+        const int c0 = hf * TQ + c;
         uint32_t v[2][16];  // product (SiLU*up: of the gate and of the up columns)
         if (live > 0) {
           tmem_ld16(lanes + oq * 64 + c0, v[0]);
@@ -775,11 +779,11 @@ __global__ void __launch_bounds__(kThreads, Expand128<R, SILU>::kCtas) lora_expa
     tc_fence_before();
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < RJ; ++j) {
 #pragma unroll
       for (int oq = 0; oq < OQ; ++oq)
         if (((on >> j) & 1u) && (SILU || (u0 + i) * 64 * OQ + oq * 64 + lc * 8 < p.N))
-          *reinterpret_cast<uint4*>(po[j] + oq * 64) = *reinterpret_cast<const uint4*>(st + oq * 16384 + so + j * 4096);
+          *reinterpret_cast<uint4*>(po[j] + oq * 64) = *reinterpret_cast<const uint4*>(st + oq * 16384 + so + j * RP * 128);
       po[j] += 64 * OQ;
     }
   }
@@ -821,7 +825,7 @@ cudaError_t launch_lora(const LoraParams& p, int C, int num_sms, cudaStream_t s)
   run = run < 2 ? 2 : run > 64 ? 64 : run;
   LoraParams q = p;
   q.units = (int)run;
-  SQ_LAUNCH((lora_expand128_kernel<R, SILU>), dim3((units + q.units - 1) / q.units, p.max_tiles), dim3(kThreads),
+  SQ_LAUNCH((lora_expand128_kernel<R, SILU>), dim3((units + q.units - 1) / q.units, p.max_tiles), dim3(TC::T),
             (size_t)TC::kSmem, s, 1, q);
   return cudaGetLastError();
 }
