@@ -417,8 +417,12 @@ __device__ __forceinline__ uint8_t* align1k(uint8_t* p) {
 // loaded from global memory, 72 us with the same behind the ring (bound by instruction issue), 61 us
 // this way (4.4 TB/s). 2048 rows, K 3584, N 37888 with the epilogue (254 MB, 39 us): 151, 62, 59 us.
 // A row's share of a unit is what the memory sees: 64-byte pieces gave 3.3 TB/s in the expand, 128
-// bytes 4.3, 256 bytes 4.7; one CTA of 16 warps per SM instead of two of 8 was slower (66 us: its
-// phases do not overlap).
+// bytes 4.3, 256 bytes 4.7. One CTA of 16 warps per SM instead of two of 8 was slower (66 us), with five
+// stages and each product one unit ahead too (2048 rows, N 37888, rank 16, 16 adapters: 100 against 73 us):
+// its phases do not overlap. Where h and the ring leave room for one CTA (rank 64 with the epilogue, rank
+// 128), 16 warps are better than 8 (107 against 115 us, 70 against 75). What did not help: products one
+// unit ahead beside two CTAs (8185 rows 71 against 65 us: fewer bytes in flight), wider pieces fetched to
+// L2 ahead (82 against 72 us), one reciprocal for four values (80 against 73 us: longer chains).
 template <int R>
 struct Shrink128 {
   static constexpr int kStage = 128 * 128 + R * 128;
@@ -733,21 +737,27 @@ lora_expand128_kernel(const LoraParams p) {
       mbar_wait(&done, (uint32_t)i & 1u, p.status, SQ_ERR_TIMEOUT_ACC);
       tc_fence_after();
     }
-    // the thread's output columns of each half of its row, 16 at a time, in place of y
+    // the thread's output columns of each half of its row, in place of y
 #pragma unroll
     for (int oq = 0; oq < OQ; ++oq) {
+      uint32_t vs[TQ / 16][2][16];  // products (SiLU*up: of the gate and of the up columns)
+      if (live > 0) {
+#pragma unroll
+        for (int c = 0; c < TQ / 16; ++c) {
+          tmem_ld16(lanes + oq * 64 + hf * TQ + c * 16, vs[c][0]);
+          if (SILU) tmem_ld16(lanes + 64 + hf * TQ + c * 16, vs[c][1]);
+        }
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int c = 0; c < TQ / 16; ++c)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) vs[c][0][k] = vs[c][1][k] = 0u;
+      }
 #pragma unroll
       for (int c = 0; c < TQ; c += 16) {
         const int c0 = hf * TQ + c;
-        uint32_t v[2][16];  // product (SiLU*up: of the gate and of the up columns)
-        if (live > 0) {
-          tmem_ld16(lanes + oq * 64 + c0, v[0]);
-          if (SILU) tmem_ld16(lanes + 64 + c0, v[1]);
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) v[0][k] = v[1][k] = 0u;
-        }
+        auto& v = vs[c / 16];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint4* at = reinterpret_cast<uint4*>(st + oq * 16384 + sw(row, c0 / 8 + h));
