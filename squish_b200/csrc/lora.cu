@@ -410,12 +410,15 @@ __device__ __forceinline__ uint8_t* align1k(uint8_t* p) {
 // shares leave h in a scratch buffer as two bf16 parts. The expand: a tile's h stays in shared memory
 // as the A operand (both parts, against the same B), y and B_s stream through a ring of 64-column units
 // (gate and up: 64 of each), and the epilogue adds the product in place of y, from where whole
-// 128-byte rows go out. The rows are gathered, so the ring is filled by cp.async, 16 bytes a thread.
+// 128-byte rows go out. The rows are gathered, so the ring is filled by cp.async, 16 bytes a thread. The
+// tiles' units, one after another, are dealt to the resident CTAs in equal shares, which the device works
+// out from the number of tiles; with runs of units from a larger grid the last CTAs ran alone (2048 rows, rank
+// 64 with the epilogue, 107 against 98 us; 4096 rows, 70 % without an adapter, 30 against 27 us).
 //
 // It is bound by bytes, so what it takes is few instructions per byte and enough bytes in flight. 8185
 // rows, K 4096, N 6144, rank up to 64 (268 MB, 42 us at the copy rate): 240 us with mma.sync fragments
-// loaded from global memory, 72 us with the same behind the ring (bound by instruction issue), 61 us
-// this way (4.4 TB/s). 2048 rows, K 3584, N 37888 with the epilogue (254 MB, 39 us): 151, 62, 59 us.
+// loaded from global memory, 72 us with the same behind the ring (bound by instruction issue), 60 us
+// this way (4.5 TB/s). 2048 rows, K 3584, N 37888 with the epilogue (254 MB, 39 us): 151, 62, 55 us.
 // A row's share of a unit is what the memory sees: 64-byte pieces gave 3.3 TB/s in the expand, 128
 // bytes 4.3, 256 bytes 4.7. One CTA of 16 warps per SM instead of two of 8 was slower (66 us), with five
 // stages and each product one unit ahead too (2048 rows, N 37888, rank 16, 16 adapters: 100 against 73 us):
@@ -611,10 +614,24 @@ lora_expand128_kernel(const LoraParams p) {
   static_assert(S >= 2 && TC::kStage % 1024 == 0, "ring");
   // The launch before this one is the shrink, which lets this one start once everything before it is
   // complete: the plan, y and B may be read at once, h after the wait.
-  const int4 tile = (int)blockIdx.y < *p.num_tiles ? p.tiles[blockIdx.y] : make_int4(-1, 0, 0, 0);
-  const int slot = tile.x, cnt = tile.z;
-  const int rank = slot >= 0 ? p.rank[slot] : 0;
-  if (cnt <= 0 || (rank <= 0 && p.in_place)) {
+  const int units = (p.N + 64 * G - 1) / (64 * G);
+  int nt = *p.num_tiles;
+  // in place, the rows without an adapter (the last tiles) are left as they are: no CTA's share holds them
+  if (p.in_place) {
+    int n = 0;
+    for (int i = threadIdx.x; i < nt; i += T) n += p.tiles[i].x >= 0;
+    __shared__ int with;
+    if (threadIdx.x == 0) with = 0;
+    __syncthreads();
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((threadIdx.x & 31) == 0) atomicAdd(&with, n);
+    __syncthreads();
+    nt = with;
+  }
+  const long long total = (long long)nt * units;
+  long long at0 = total * blockIdx.x / gridDim.x;
+  const long long at1 = total * (blockIdx.x + 1) / gridDim.x;
+  if (at0 >= at1) {
     pdl_wait();
     pdl_trigger();
     return;
@@ -626,7 +643,6 @@ lora_expand128_kernel(const LoraParams p) {
   __shared__ __align__(8) uint64_t done;
   __shared__ uint32_t tmem_slot;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid < 128) rows[tid] = tid < cnt ? p.order[tile.y + tid] : -1;
   if (tid == 0) {
     mbar_init(&done, 1);
     fence_mbar_init();
@@ -639,166 +655,186 @@ lora_expand128_kernel(const LoraParams p) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int live = rank <= 0 ? 0 : min(R, (rank + 15) / 16 * 16);
-  const int units = (p.N + 64 * G - 1) / (64 * G);
-  const int u0 = blockIdx.x * p.units, n2 = min(p.units, units - u0);
+  bool waited = false;
+  uint32_t phase = 0;  // of the next product
 
-  // a thread copies chunk tid % 8 of rows tid / 8 + RP j of y (and of out), and pieces of B rows
-  const int lr = tid >> 3, lc = tid & 7;
-  const __nv_bfloat16* py[RJ];
-  __nv_bfloat16* po[RJ];
-  unsigned on = 0;
+  while (at0 < at1) {  // a tile's part of this CTA's share: units u0 .. u0 + n2
+    const int ti = (int)(at0 / units);
+    const int u0 = (int)(at0 - (long long)ti * units), n2 = (int)min((long long)(units - u0), at1 - at0);
+    at0 += n2;
+    const int4 tile = p.tiles[ti];
+    const int slot = tile.x, cnt = tile.z;
+    const int rank = slot >= 0 ? p.rank[slot] : 0;
+    if (rank <= 0 && p.in_place) continue;
+    const int live = rank <= 0 ? 0 : min(R, (rank + 15) / 16 * 16);
+    if (tid < 128) rows[tid] = tid < cnt ? p.order[tile.y + tid] : -1;
+    __syncthreads();
+
+    // a thread copies chunk tid % 8 of rows tid / 8 + RP j of y (and of out), and pieces of B rows
+    const int lr = tid >> 3, lc = tid & 7;
+    const __nv_bfloat16* py[RJ];
+    __nv_bfloat16* po[RJ];
+    unsigned on = 0;
 #pragma unroll
-  for (int j = 0; j < RJ; ++j) {
-    const int r = rows[lr + RP * j];
-    on |= (r >= 0 ? 1u : 0u) << j;
-    py[j] = p.y + (r < 0 ? 0 : r) * p.ldy + (long long)u0 * 64 * G + lc * 8;
-    po[j] = p.out + (r < 0 ? 0 : r) * p.ldo + (long long)u0 * 64 * OQ + lc * 8;
-  }
-  constexpr int CH = R / 8;          // 16-byte pieces of a B row
-  constexpr int BN = T / CH;         // B rows per pass
-  const int bn = tid / CH, bc = tid % CH;
-  const __nv_bfloat16* pb = p.b + ((size_t)(slot < 0 ? 0 : slot) * p.N + (size_t)u0 * 64 * G + bn) * R + bc * 8;
-  const int so = sw(lr, lc);
-  int col = u0 * 64 * G, wr = 0;  // the unit's first column; next stage to fill
-  auto issue = [&](int i) {
-    uint8_t* st = ring + wr * TC::kStage;
-    wr = wr == S - 1 ? 0 : wr + 1;
-    if (i < n2) {
+    for (int j = 0; j < RJ; ++j) {
+      const int r = rows[lr + RP * j];
+      on |= (r >= 0 ? 1u : 0u) << j;
+      py[j] = p.y + (r < 0 ? 0 : r) * p.ldy + (long long)u0 * 64 * G + lc * 8;
+      po[j] = p.out + (r < 0 ? 0 : r) * p.ldo + (long long)u0 * 64 * OQ + lc * 8;
+    }
+    constexpr int CH = R / 8;          // 16-byte pieces of a B row
+    constexpr int BN = T / CH;         // B rows per pass
+    const int bn = tid / CH, bc = tid % CH;
+    const __nv_bfloat16* pb = p.b + ((size_t)(slot < 0 ? 0 : slot) * p.N + (size_t)u0 * 64 * G + bn) * R + bc * 8;
+    const int so = sw(lr, lc);
+    int col = u0 * 64 * G, wr = 0;  // the unit's first column; next stage to fill
+    auto issue = [&](int i) {
+      uint8_t* st = ring + wr * TC::kStage;
+      wr = wr == S - 1 ? 0 : wr + 1;
+      if (i < n2) {
+#pragma unroll
+        for (int j = 0; j < RJ; ++j) {
+#pragma unroll
+          for (int q = 0; q < G; ++q) {
+            const bool in = SILU || col + q * 64 + lc * 8 < p.N;
+            cp16(st + q * 16384 + so + j * RP * 128, in ? py[j] + q * 64 : p.y, in && ((on >> j) & 1u));
+          }
+          py[j] += 64 * G;
+        }
+        if (bc * 8 < live) {
+#pragma unroll
+          for (int k = 0; k < G * 64; k += BN) {
+            const int n = bn + k;
+            if (BN > G * 64 && n >= G * 64) break;
+            const bool ok = SILU || col + n < p.N;
+            const int at = TC::kPair ? sw(n & 63, (n >> 6) * 4 + bc) : (bc >> 3) * (G * 8192) + sw(n, bc & 7);
+            cp16(st + G * 16384 + at, ok ? pb + (size_t)k * R : p.b, ok);
+          }
+        }
+        pb += (size_t)64 * G * R;
+        col += 64 * G;
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) issue(i);
+    if (!waited) {
+      pdl_wait();
+      pdl_trigger();
+      waited = true;
+    }
+    if (live > 0) {  // h of the tile, as the A operand
+      for (int e = tid; e < 128 * 2 * CH; e += T) {
+        const int r = e / (2 * CH), q = e / CH % 2, c = e % CH;
+        if (c * 8 < live) {
+          const int at = R >= 64 ? (q * (R / 64) + (c >> 3)) * 16384 + sw(r, c & 7) : sw(r, q * CH + c);
+          cp16(ha + at, r < cnt ? p.h + ((size_t)(tile.y + r) * 2 + q) * R + c * 8 : p.h, r < cnt);
+        }
+      }
+    }
+    cp_commit();
+    constexpr int TQ = 8192 / T;                             // columns of a half per thread
+    const int row = (warp & 3) * 32 + lane, hf = warp >> 2;  // this thread's row and part of the columns
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    constexpr uint32_t idesc = idesc_bf16_f32(128, TC::kPair ? 64 : 64 * G);
+    int rd = 0;
+    for (int i = 0; i < n2; ++i) {
+      if (i == 0) cp_wait<0>();
+      else cp_wait<S - 2>();
+      fence_proxy_async_smem();
+      __syncthreads();
+      uint8_t* st = ring + rd * TC::kStage;
+      rd = rd == S - 1 ? 0 : rd + 1;
+      if (live > 0 && warp == 0) {
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t a = smem_u32(ha), b = smem_u32(st + G * 16384);
+#pragma unroll
+          for (int g = 0; g < (TC::kPair ? 2 : 1); ++g)  // (gate, up)
+#pragma unroll
+            for (int q = 1; q >= 0; --q)  // lower part first
+              for (int ks = 0; ks < live / 16; ++ks) {
+                const uint32_t ao = R >= 64 ? (q * (R / 64) + (ks >> 2)) * 16384 + (ks & 3) * 32 : (q * R / 16 + ks) * 32;
+                const uint32_t bo = TC::kPair ? g * 64 + ks * 32 : (ks >> 2) * (G * 8192) + (ks & 3) * 32;
+                mma_bf16_ss(tmem + g * 64, sdesc_sw128(a + ao), sdesc_sw128(b + bo), idesc, q == 0 || ks > 0 ? 1u : 0u);
+              }
+          mma_commit(&done);
+        }
+        __syncwarp();
+      }
+      issue(i + S - 1);  // (its stage was emptied by the step before this one)
+      if (live > 0) {
+        mbar_wait(&done, phase, p.status, SQ_ERR_TIMEOUT_ACC);
+        phase ^= 1u;
+        tc_fence_after();
+      }
+      // the thread's output columns of each half of its row, in place of y
+#pragma unroll
+      for (int oq = 0; oq < OQ; ++oq) {
+        uint32_t vs[TQ / 16][2][16];  // products (SiLU*up: of the gate and of the up columns)
+        if (live > 0) {
+#pragma unroll
+          for (int c = 0; c < TQ / 16; ++c) {
+            tmem_ld16(lanes + oq * 64 + hf * TQ + c * 16, vs[c][0]);
+            if (SILU) tmem_ld16(lanes + 64 + hf * TQ + c * 16, vs[c][1]);
+          }
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int c = 0; c < TQ / 16; ++c)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) vs[c][0][k] = vs[c][1][k] = 0u;
+        }
+#pragma unroll
+        for (int c = 0; c < TQ; c += 16) {
+          const int c0 = hf * TQ + c;
+          auto& v = vs[c / 16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint4* at = reinterpret_cast<uint4*>(st + oq * 16384 + sw(row, c0 / 8 + h));
+            const uint4 y = *at;
+            const uint32_t yw[4] = {y.x, y.y, y.z, y.w};
+            uint32_t uw[4] = {0, 0, 0, 0};
+            if (SILU) {
+              const uint4 x = *reinterpret_cast<const uint4*>(st + 16384 + sw(row, c0 / 8 + h));
+              uw[0] = x.x;
+              uw[1] = x.y;
+              uw[2] = x.z;
+              uw[3] = x.w;
+            }
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float f0 = lo_f(yw[k]) + __uint_as_float(v[0][8 * h + 2 * k]);
+              float f1 = hi_f(yw[k]) + __uint_as_float(v[0][8 * h + 2 * k + 1]);
+              if (SILU) {
+                f0 = silu_mul(f0, lo_f(uw[k]) + __uint_as_float(v[1][8 * h + 2 * k]));
+                f1 = silu_mul(f1, hi_f(uw[k]) + __uint_as_float(v[1][8 * h + 2 * k + 1]));
+              }
+              o[k] = pack_bf16(f0, f1);
+            }
+            *at = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncthreads();
 #pragma unroll
       for (int j = 0; j < RJ; ++j) {
 #pragma unroll
-        for (int q = 0; q < G; ++q) {
-          const bool in = SILU || col + q * 64 + lc * 8 < p.N;
-          cp16(st + q * 16384 + so + j * RP * 128, in ? py[j] + q * 64 : p.y, in && ((on >> j) & 1u));
-        }
-        py[j] += 64 * G;
-      }
-      if (bc * 8 < live) {
-#pragma unroll
-        for (int k = 0; k < G * 64; k += BN) {
-          const int n = bn + k;
-          if (BN > G * 64 && n >= G * 64) break;
-          const bool ok = SILU || col + n < p.N;
-          const int at = TC::kPair ? sw(n & 63, (n >> 6) * 4 + bc) : (bc >> 3) * (G * 8192) + sw(n, bc & 7);
-          cp16(st + G * 16384 + at, ok ? pb + (size_t)k * R : p.b, ok);
-        }
-      }
-      pb += (size_t)64 * G * R;
-      col += 64 * G;
-    }
-    cp_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < S - 1; ++i) issue(i);
-  pdl_wait();
-  pdl_trigger();
-  if (live > 0) {  // h of the tile, as the A operand
-    for (int e = tid; e < 128 * 2 * CH; e += T) {
-      const int r = e / (2 * CH), q = e / CH % 2, c = e % CH;
-      if (c * 8 < live) {
-        const int at = R >= 64 ? (q * (R / 64) + (c >> 3)) * 16384 + sw(r, c & 7) : sw(r, q * CH + c);
-        cp16(ha + at, r < cnt ? p.h + ((size_t)(tile.y + r) * 2 + q) * R + c * 8 : p.h, r < cnt);
+        for (int oq = 0; oq < OQ; ++oq)
+          if (((on >> j) & 1u) && (SILU || (u0 + i) * 64 * OQ + oq * 64 + lc * 8 < p.N))
+            *reinterpret_cast<uint4*>(po[j] + oq * 64) = *reinterpret_cast<const uint4*>(st + oq * 16384 + so + j * RP * 128);
+        po[j] += 64 * OQ;
       }
     }
-  }
-  cp_commit();
-  constexpr int TQ = 8192 / T;                             // columns of a half per thread
-  const int row = (warp & 3) * 32 + lane, hf = warp >> 2;  // this thread's row and part of the columns
-  const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-  constexpr uint32_t idesc = idesc_bf16_f32(128, TC::kPair ? 64 : 64 * G);
-  int rd = 0;
-  for (int i = 0; i < n2; ++i) {
-    if (i == 0) cp_wait<0>();
-    else cp_wait<S - 2>();
-    fence_proxy_async_smem();
+    cp_wait<0>();
     __syncthreads();
-    uint8_t* st = ring + rd * TC::kStage;
-    rd = rd == S - 1 ? 0 : rd + 1;
-    if (live > 0 && warp == 0) {
-      tc_fence_after();
-      if (elect_one()) {
-        const uint32_t a = smem_u32(ha), b = smem_u32(st + G * 16384);
-#pragma unroll
-        for (int g = 0; g < (TC::kPair ? 2 : 1); ++g)  // (gate, up)
-#pragma unroll
-          for (int q = 1; q >= 0; --q)  // lower part first
-            for (int ks = 0; ks < live / 16; ++ks) {
-              const uint32_t ao = R >= 64 ? (q * (R / 64) + (ks >> 2)) * 16384 + (ks & 3) * 32 : (q * R / 16 + ks) * 32;
-              const uint32_t bo = TC::kPair ? g * 64 + ks * 32 : (ks >> 2) * (G * 8192) + (ks & 3) * 32;
-              mma_bf16_ss(tmem + g * 64, sdesc_sw128(a + ao), sdesc_sw128(b + bo), idesc, q == 0 || ks > 0 ? 1u : 0u);
-            }
-        mma_commit(&done);
-      }
-      __syncwarp();
-    }
-    issue(i + S - 1);  // (its stage was emptied by the step before this one)
-    if (live > 0) {
-      mbar_wait(&done, (uint32_t)i & 1u, p.status, SQ_ERR_TIMEOUT_ACC);
-      tc_fence_after();
-    }
-    // the thread's output columns of each half of its row, in place of y
-#pragma unroll
-    for (int oq = 0; oq < OQ; ++oq) {
-      uint32_t vs[TQ / 16][2][16];  // products (SiLU*up: of the gate and of the up columns)
-      if (live > 0) {
-#pragma unroll
-        for (int c = 0; c < TQ / 16; ++c) {
-          tmem_ld16(lanes + oq * 64 + hf * TQ + c * 16, vs[c][0]);
-          if (SILU) tmem_ld16(lanes + 64 + hf * TQ + c * 16, vs[c][1]);
-        }
-        tmem_wait_ld();
-      } else {
-#pragma unroll
-        for (int c = 0; c < TQ / 16; ++c)
-#pragma unroll
-          for (int k = 0; k < 16; ++k) vs[c][0][k] = vs[c][1][k] = 0u;
-      }
-#pragma unroll
-      for (int c = 0; c < TQ; c += 16) {
-        const int c0 = hf * TQ + c;
-        auto& v = vs[c / 16];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint4* at = reinterpret_cast<uint4*>(st + oq * 16384 + sw(row, c0 / 8 + h));
-          const uint4 y = *at;
-          const uint32_t yw[4] = {y.x, y.y, y.z, y.w};
-          uint32_t uw[4] = {0, 0, 0, 0};
-          if (SILU) {
-            const uint4 x = *reinterpret_cast<const uint4*>(st + 16384 + sw(row, c0 / 8 + h));
-            uw[0] = x.x;
-            uw[1] = x.y;
-            uw[2] = x.z;
-            uw[3] = x.w;
-          }
-          uint32_t o[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float f0 = lo_f(yw[k]) + __uint_as_float(v[0][8 * h + 2 * k]);
-            float f1 = hi_f(yw[k]) + __uint_as_float(v[0][8 * h + 2 * k + 1]);
-            if (SILU) {
-              f0 = silu_mul(f0, lo_f(uw[k]) + __uint_as_float(v[1][8 * h + 2 * k]));
-              f1 = silu_mul(f1, hi_f(uw[k]) + __uint_as_float(v[1][8 * h + 2 * k + 1]));
-            }
-            o[k] = pack_bf16(f0, f1);
-          }
-          *at = make_uint4(o[0], o[1], o[2], o[3]);
-        }
-      }
-    }
-    tc_fence_before();
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < RJ; ++j) {
-#pragma unroll
-      for (int oq = 0; oq < OQ; ++oq)
-        if (((on >> j) & 1u) && (SILU || (u0 + i) * 64 * OQ + oq * 64 + lc * 8 < p.N))
-          *reinterpret_cast<uint4*>(po[j] + oq * 64) = *reinterpret_cast<const uint4*>(st + oq * 16384 + so + j * RP * 128);
-      po[j] += 64 * OQ;
-    }
   }
-  cp_wait<0>();
-  __syncthreads();
+  if (!waited) {
+    pdl_wait();
+    pdl_trigger();
+  }
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, TC::kCols);
@@ -829,14 +865,11 @@ cudaError_t launch_lora(const LoraParams& p, int C, int num_sms, cudaStream_t s)
   using TC = Expand128<R, SILU>;
   e = allow_smem(lora_expand128_kernel<R, SILU>, TC::kSmem);
   if (e != cudaSuccess) return e;
-  // runs of units: about three CTAs per resident one, so that the last ones level out
+  // the tiles' units in equal shares
   const int units = (p.N + 64 * TC::G - 1) / (64 * TC::G);
-  long long run = (long long)p.max_tiles * units / (3ll * TC::kCtas * num_sms);
-  run = run < 2 ? 2 : run > 64 ? 64 : run;
-  LoraParams q = p;
-  q.units = (int)run;
-  SQ_LAUNCH((lora_expand128_kernel<R, SILU>), dim3((units + q.units - 1) / q.units, p.max_tiles), dim3(TC::T),
-            (size_t)TC::kSmem, s, 1, q);
+  const long long work = (long long)p.max_tiles * units;
+  const int ctas = (int)(work < 2ll * TC::kCtas * num_sms ? (work + 1) / 2 : TC::kCtas * num_sms);
+  SQ_LAUNCH((lora_expand128_kernel<R, SILU>), dim3(ctas), dim3(TC::T), (size_t)TC::kSmem, s, 1, p);
   return cudaGetLastError();
 }
 

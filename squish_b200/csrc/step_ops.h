@@ -115,7 +115,6 @@ struct LoraParams {
   int M, K, N, R, tm, max_tiles;
   bool silu, in_place;
   __nv_bfloat16* h;  // [M, 2, R] scratch (tiles of 128 rows): scale * A x of every position, upper and lower part
-  int units;         // (set by the launch) column units of a CTA
   int* status;
 };
 cudaError_t lora_add_launch(const LoraParams& p, int num_sms, cudaStream_t s);

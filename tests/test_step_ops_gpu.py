@@ -589,6 +589,26 @@ def test_lora_special_values_stay_in_their_rows(cuda):
     assert ok[keep].all()
 
 
+@pytest.mark.parametrize("n,rank", [(128, 16), (2176, 16), (2176, 64), (640, 128)])
+@pytest.mark.parametrize("silu", [False, True])
+def test_lora_empty_slots_between_full_ones(cuda, n, rank, silu):
+    """Large steps: tiles that are left as they are, first, between others and last, in place and not."""
+    m, k, slots = 900, 72, 6
+    pool, ads = make_adapters(cuda, slots, k, n, rank)
+    for s in (0, 2, 3):
+        pool.clear(s)
+        ads.pop(s, None)
+    g = torch.Generator().manual_seed(n + rank)
+    rows = torch.randint(-1, slots, (m,), generator=g)
+    x, y = torch.randn(m, k, generator=g).to(BF), torch.randn(m, n, generator=g).to(BF)
+    for r in (rows, torch.full_like(rows, 2), torch.full_like(rows, -1), torch.where(rows < 4, -1, rows)):
+        plan = ops.lora_plan(r.to(torch.int32).to(cuda), slots)
+        yc = y.to(cuda)
+        out = ops.lora_add(x.to(cuda), pool, plan, yc, out=None if silu else yc, silu_mul=silu)
+        want, tol = lora_ref(x, y, r, ads, silu)
+        assert ((out.double().cpu() - want).abs() <= tol).all()
+
+
 def test_lora_plan_reports_bad_slots(cuda):
     rows = i32([0, 5, -2, 1, 2**31 - 1, -1], cuda)
     plan = ops.lora_plan(rows, 2)
