@@ -12,8 +12,8 @@
 // keys plus a ballot. Without a bias the choice follows the logits themselves (both scores are
 // monotone in them): no rounding can reorder it. With a bias, fp32 values cut the row to a short
 // list (with a margin for their error) whose exact values, one fp64 score per lane, are compared.
-// Group scores are compared in fp32; where the last open and the first closed group lie within the
-// error bound the same warp ranks the groups again in fp64. So the ids are those of the exact scores.
+// Group scores are compared in fp32; where an open and a closed group lie within their own error
+// bounds the same warp ranks the groups again in fp64. So the ids are those of the exact scores.
 //
 // What bounds a large step is instruction issue (some 900 instructions per token; 16384 tokens, 256
 // experts in 8 groups, top 8, bf16: 23 us for 9.4 MB): scores and group sums 10 us of it, the short list
@@ -108,22 +108,26 @@ __device__ __forceinline__ void group_top2(const S (&v)[EPL], const Shape& sh, i
   }
 }
 
-// Open groups by score (lane g < groups: gscore). sure: false when the last open and the first closed
-// group lie within tol (1 + |score|) of each other; tol < 0: the scores are exact.
-__device__ __forceinline__ unsigned open_groups32(float gscore, const Shape& sh, int lane, float tol, bool& sure) {
+// Open groups by score (lane g < groups: gscore, off by at most err). sure: false when an open and a closed
+// group's exact scores may be the other way round; err < 0: the scores are exact.
+__device__ __forceinline__ unsigned open_groups32(float gscore, const Shape& sh, int lane, float err, bool& sure) {
   uint32_t gk = lane < sh.groups ? ord32(clean(gscore)) : 0u;
   unsigned open = 0;
-  uint32_t last = 0;
   for (int g = 0; g < sh.top_groups; ++g) {
-    last = __reduce_max_sync(kFull, gk);
-    const int win = __ffs(__ballot_sync(kFull, gk == last)) - 1;
+    const uint32_t best = __reduce_max_sync(kFull, gk);
+    const int win = __ffs(__ballot_sync(kFull, gk == best)) - 1;
     open |= 1u << win;
     if (lane == win) gk = 0u;
   }
   sure = true;
-  if (tol >= 0.f && sh.top_groups < sh.groups) {
-    const float a = unord32(last), b = unord32(__reduce_max_sync(kFull, gk));
-    sure = a - b > tol * (1.f + fabsf(a));
+  if (err >= 0.f && sh.top_groups < sh.groups) {  // (one case for the whole warp)
+    // the least that an open group's score can be against the most that a closed one's can be (NaN, of an
+    // infinite error: anything)
+    const bool in = (open >> lane) & 1u;
+    const float low = gscore - err, high = gscore + err;
+    const uint32_t lo = __reduce_min_sync(kFull, in ? ord32(clean(low)) : 0xffffffffu);
+    const uint32_t hi = __reduce_max_sync(kFull, !in && lane < sh.groups ? ord32(high == high ? high : INFINITY) : 0u);
+    sure = lo > hi;
   }
   return open;
 }
@@ -373,11 +377,13 @@ __global__ void __launch_bounds__(kWarps * 32) route_scored_kernel(const RouteSc
     for (int o = 16; o; o >>= 1) z64 += __shfl_xor_sync(kFull, z64, o);
     inv_z64 = z64 > 0.0 ? 1.0 / z64 : 0.0;
   }
-  // fp32 choice values. A score (absolute value <= 1) is off by less than 2e-7 (argument rounded by
-  // 2^-24 of itself, exponential 2 ulp, reciprocal 1 ulp: times s (1 - s), 2e-7), adding the bias rounds
-  // by 2^-24 of the sum. A difference of two sums of two is off by at most 4 (2e-7 + 6e-8 |c|) + 2 * 6e-8
-  // |sum| < 1e-6 (1 + |sum|), one of two values by half as much.
-  constexpr float kTol = 1e-6f;
+  // fp32 choice values. A score (absolute value <= 1) is off by less than 2.5e-7 (argument rounded by
+  // 2^-24 of itself, exponential 2 ulp, reciprocal 1 ulp: times s (1 - s)), adding the bias rounds by 2^-24
+  // of the sum. Two values that are compared are off by less than 5e-7 + 1.2e-7 |c| together, within the
+  // margin of kTol (1 + |c|) of a list. A group's sum of two is off by 5e-7 + 2^-24 (|c1| + |c2| + |sum|), and
+  // its distance to the error's ends rounds by 2^-24 |sum| more: less than kSumErr + kSumRel (|c1| + |c2|).
+  // (The operands count, not the sum: biases of opposite signs cancel in it, their roundings do not.)
+  constexpr float kTol = 1e-6f, kSumErr = 5e-7f, kSumRel = 2e-7f;
   float c[EPL];
   if (p.bias == nullptr) {
 #pragma unroll
@@ -404,19 +410,23 @@ __global__ void __launch_bounds__(kWarps * 32) route_scored_kernel(const RouteSc
   }
   unsigned open = kFull;
   if (sh.groups > 1) {
-    float g1, g2, g, tol = -1.f;
+    float g1, g2, g, err = -1.f;
     group_top2<EPL, float>(c, sh, lane, reinterpret_cast<float*>(buf), g1, g2);
     g = g1;
-    if (p.bias != nullptr) tol = kTol;
     if (sh.top2 && sh.gsize > 1) {
-      g = g1 + g2;
-      if (p.bias == nullptr)
-        g = (g1 == kNegInf ? 0.f : sigm ? sigmoid_fast(g1) : (g1 == m ? 1.f : exp_fast(g1 - m))) +
-            (g2 == kNegInf ? 0.f : sigm ? sigmoid_fast(g2) : (g2 == m ? 1.f : exp_fast(g2 - m)));
-      tol = kTol;
+      float s1 = g1, s2 = g2;
+      if (p.bias == nullptr) {
+        s1 = g1 == kNegInf ? 0.f : sigm ? sigmoid_fast(g1) : (g1 == m ? 1.f : exp_fast(g1 - m));
+        s2 = g2 == kNegInf ? 0.f : sigm ? sigmoid_fast(g2) : (g2 == m ? 1.f : exp_fast(g2 - m));
+      }
+      g = clean(s1 + s2);
+      // (an infinite value makes an infinite sum, which is exact)
+      err = s1 < INFINITY && s2 > kNegInf ? kSumErr + kSumRel * (fabsf(s1) + fabsf(s2)) : 0.f;
+    } else if (p.bias != nullptr) {
+      err = fabsf(g) < INFINITY ? kSumErr + kSumRel * fabsf(g) : 0.f;
     }
     bool sure;
-    open = open_groups32(g, sh, lane, tol, sure);
+    open = open_groups32(g, sh, lane, err, sure);
     if (!sure) open = open_groups64<EPL>(x, c, g1, g2, kTol, p.bias, sigm, m, inv_z64, sh, lane, buf);
   }
   uint32_t k[EPL];
