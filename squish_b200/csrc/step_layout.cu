@@ -7,6 +7,7 @@
 //
 // Every block scans the lengths of all sequences itself (8 bytes each, from L2) and then writes its
 // share of the token, tile and page rows, found by binary search in the prefixes in shared memory.
+// A sequence whose tokens do not all fit rests (kv_len of what it had, tiles that are padding).
 // No block needs another's result: the page of a new token comes from the free list, not from the
 // table entry that another block may be writing. So the step is one launch with no grid-wide wait.
 // What bounds it is latency: launch, lengths, scan, search, page, slot (64 sequences: 3.5 us for 3 KB;
@@ -100,14 +101,23 @@ __global__ void __launch_bounds__(kThreads) step_layout_kernel(const StepLayoutP
   if (tid == 0) qs[0] = pg[0] = ts[0] = 0;
   __syncthreads();
   const int T = (int)qs[B], P = (int)pg[B], NT = (int)ts[B];
+  // Rows, pages and table columns for all of a sequence's tokens? What reads the cache goes by kv_len and
+  // the tiles: past a missing page lies what another request stored, past the row's width another row.
+  const unsigned held = (unsigned)min((long long)p.bt_width * ps, 0xffffffffll);  // tokens of a full table row
+  auto fits = [&](int b) -> bool {
+    return qs[b + 1] <= (unsigned)p.token_cap && (pg[b + 1] == pg[b] || pg[b + 1] <= (unsigned)p.n_free) &&
+           (unsigned)ctx[b] + (qs[b + 1] - qs[b]) <= held;
+  };
   if (blockIdx.x == 0) {
     if (T > p.token_cap || NT > p.tile_cap || P > p.n_free) bad = true;
     for (int b = tid; b <= B; b += kThreads) {
       p.q_start[b] = (int)qs[b];
       if (b == B) break;
       const int q = (int)(qs[b + 1] - qs[b]);
-      p.kv_len[b] = ctx[b] + q;
-      p.last_row[b] = q > 0 && (int)qs[b + 1] <= p.token_cap ? (int)qs[b + 1] - 1 : -1;
+      const bool whole = fits(b);
+      if ((unsigned)ctx[b] > held) bad = true;
+      p.kv_len[b] = whole ? ctx[b] + q : (int)min((unsigned)ctx[b], held);
+      p.last_row[b] = whole && q > 0 ? (int)qs[b + 1] - 1 : -1;
     }
     if (tid == 0) {
       p.totals[0] = T;
@@ -172,8 +182,11 @@ __global__ void __launch_bounds__(kThreads) step_layout_kernel(const StepLayoutP
   for (int i = first; i < p.tile_cap; i += stride) {
     int seq = 0, q0 = kLayoutPadQ0;
     if (i < NT) {
-      seq = upper(ts, B, (unsigned)i);
-      q0 = (i - (int)ts[seq]) * p.tile;
+      const int b = upper(ts, B, (unsigned)i);
+      if (fits(b)) {
+        seq = b;
+        q0 = (i - (int)ts[b]) * p.tile;
+      }
     }
     p.tile_seq[i] = seq;
     p.tile_q0[i] = q0;

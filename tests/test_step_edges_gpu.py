@@ -1,12 +1,16 @@
 """Edges of the serving-step operators (squish_b200.ops.step) on the GPU: each test is a call that the
 documentation allows, or a refusal, next to the limits of an operator."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
 from squish_b200 import ops
+from squish_b200.ops import kernels as K
 
-from ._step_refs import route_ref
+from ._step_refs import PAD_Q0, route_ref
+from .test_step_ops_gpu import BF, i32, status
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +49,84 @@ def test_group_sums_of_opposite_biases_are_ranked_exactly(cuda, B, score, groups
     ops.moe_route_scored(x.to(cuda), k, ids, w, bias=bias.to(cuda), **kw)
     want, _ = route_ref(x, k, bias=bias, **kw)
     assert np.array_equal(ids.view(T, k).cpu().numpy(), want)
+
+
+# ----------------------------------------------------------------------------- layout
+def test_layout_sequences_that_do_not_fit_keep_their_length(cuda):
+    """Without pages, table columns or rows for all of its tokens a sequence rests: kv_len is that of the
+    pages it has, last_row -1, its attention tiles padding; the others are as without it."""
+    def run(ctx, q, tab, free, cap=32, width=2):
+        lay = ops.StepLayout(len(ctx), cap, device=cuda)
+        ops.step_layout(i32(ctx, cuda), i32(q, cuda), tab, i32(free, cuda), 4, lay)
+        n = lay.totals.tolist()[2]
+        return lay, list(zip(lay.tile_seq.tolist(), lay.tile_q0.tolist()))[:n]
+
+    full = lambda b, w=2: torch.full((b, w), -9, dtype=torch.int32, device=cuda)  # noqa: E731
+    # one page left, the first sequence takes it; the second, with 3 tokens cached, needs two more
+    tab = full(3, 3)
+    tab[1, 0], tab[2, 0] = 7, 8
+    lay, tiles = run([0, 3, 1], [4, 8, 2], tab, [5])
+    assert lay.kv_len.tolist() == [4, 3, 3] and lay.last_row.tolist() == [3, -1, 13] and status(cuda) == 6
+    assert tiles == [(0, 0), (0, PAD_Q0), (2, 0)] and tab.tolist()[0][0] == 5 and tab.tolist()[1] == [7, -9, -9]
+    # a table row too narrow for the new tokens
+    lay, tiles = run([3, 1], [6, 1], torch.tensor([[1, -9], [2, -9]], dtype=torch.int32, device=cuda), [4, 3])
+    assert lay.kv_len.tolist() == [3, 2] and lay.last_row.tolist() == [-1, 6] and status(cuda) == 6
+    assert tiles == [(0, PAD_Q0), (1, 0)]
+    # a resting sequence whose context its table row cannot hold: no more than the row's pages
+    lay, _ = run([100, 8], [0, 0], full(2), [])
+    assert lay.kv_len.tolist() == [8, 8] and lay.last_row.tolist() == [-1, -1] and status(cuda) == 6
+    lay, _ = run([8, 8], [0, 0], full(2), [])
+    assert lay.kv_len.tolist() == [8, 8] and status(cuda) == 0
+    # more tokens than rows: sequences past the buffers rest, q_start tells the rows that were asked for
+    lay, tiles = run([0, 2, 1], [3, 3, 2], torch.ones(3, 2, dtype=torch.int32, device=cuda), [1, 2, 3], cap=4)
+    assert lay.kv_len.tolist() == [3, 2, 1] and lay.last_row.tolist() == [2, -1, -1] and status(cuda) == 6
+    assert tiles == [(0, 0), (0, PAD_Q0), (0, PAD_Q0)]
+    # sums past 32 bits
+    lay, _ = run([2] * 4, [2**30] * 4, full(4), [1], cap=4)
+    assert lay.kv_len.tolist() == [2] * 4 and lay.last_row.tolist() == [-1] * 4 and status(cuda) == 6
+
+
+def paged(cuda, pages, hkv, ps, d, seed):
+    """bf16 KV pages with values, and [pages * ps, hkv, d] views of keys and values."""
+    g = torch.Generator().manual_seed(seed)
+    kv = [torch.randn(pages, hkv, ps, d, generator=g).to(BF).to(cuda) for _ in range(2)]
+    codes = [t.view(torch.uint8).view(pages, hkv, ps, 2 * d) for t in kv]
+    scales = [torch.zeros(pages, hkv, ps, 1, dtype=torch.float16, device=cuda) for _ in range(2)]
+    return (codes[0], scales[0], codes[1], scales[1]), kv
+
+
+def attend(q, k, v, n):
+    """Rows of one query [hq * d] over the first n keys and values [*, hkv, d], in 64 bits, and the error of
+    probabilities in bf16 (2^-8 of the mass of |v|, its sums far below) and of the output in bf16."""
+    d = k.shape[-1]
+    q = q.double().cpu().view(-1, d)
+    kk, vv = (t[:n].double().cpu().repeat_interleave(q.shape[0] // t.shape[1], 1) for t in (k, v))
+    p = torch.softmax(torch.einsum("hd,khd->hk", q, kk) / math.sqrt(d), -1)
+    out = torch.einsum("hk,khd->hd", p, vv).reshape(-1)
+    return out, 2.0**-7 * torch.einsum("hk,khd->hd", p, vv.abs()).reshape(-1) + 2.0**-8 * out.abs() + 2.0**-12
+
+
+def test_attention_reads_no_page_that_a_sequence_did_not_get(cuda):
+    """The free list runs out: the table entries behind a sequence's pages still name pages that belong to
+    others, and neither attention kernel looks at them."""
+    hq, hkv, d, ps, pages = 4, 2, 64, 16, 6
+    cache, kv = paged(cuda, pages, hkv, ps, d, 3)
+    fk, fv = K.KV_FORMATS["bf16"]
+    x = torch.randn(64, hq * d, generator=torch.Generator().manual_seed(4)).to(BF).to(cuda)
+    # (sequence 0 has pages 0 and 1; sequence 1 has page 2 for its 16 tokens, then a stale entry, page 1)
+    tab = torch.tensor([[0, 1, -1], [2, 1, 0]], dtype=torch.int32, device=cuda)
+    rows = [t[[2]].transpose(1, 2).reshape(ps, hkv, d) for t in kv]
+    lay = ops.StepLayout(2, 64, device=cuda)
+    ops.step_layout(i32([31, 16], cuda), i32([1, 1], cuda), tab, i32([], cuda), ps, lay)
+    assert status(cuda) == 6 and lay.kv_len.tolist() == [32, 16] and lay.last_row.tolist() == [0, -1]
+    out = torch.zeros(2, hq * d, dtype=BF, device=cuda)
+    ops.paged_decode_attention(x[:2], *cache, tab, lay.kv_len, out, hq, hkv, d, ps, 32, fk, fv, 1 / math.sqrt(d), 64)
+    want, tol = attend(x[1], *rows, 16)
+    assert ((out[1].double().cpu() - want).abs() <= tol).all()
+    q = i32([1, 20], cuda)
+    ops.step_layout(i32([31, 16], cuda), q, tab, i32([], cuda), ps, lay)
+    out = torch.full((64, hq * d), 3.0, dtype=BF, device=cuda)
+    ops.paged_prefill_attention(x, *cache, tab, lay.tile_seq, lay.tile_q0, lay.q_start[:2], q, lay.kv_len,
+                                lay.tile_seq.numel(), out, hq, hkv, d, ps, 32, fk, fv, 1 / math.sqrt(d))
+    assert (out[1:] == 3).all() and not (out[0] == 3).all()
+    assert status(cuda) == 6
