@@ -209,7 +209,9 @@ cudaError_t step_layout_launch(const StepLayoutParams& p, int num_sms, cudaStrea
   // 4.9), four from there on (1000 sequences, 250000 tokens: 6.8 us against 8.4).
   const int v = p.token_cap > 65536 ? 4 : 1;
   auto* kern = v == 4 ? step_layout_kernel<4> : step_layout_kernel<1>;
-  if (smem > 48 * 1024) {
+  // (the kernel's static arrays count towards the 48 KB that need no permission: 3066 to 3071 sequences
+  // stay below it with their prefixes alone)
+  if (smem > 47 * 1024) {
     const cudaError_t e = allow_smem(kern, 4 * (4 * kLayoutMaxSeqs + 3));
     if (e != cudaSuccess) return e;
   }

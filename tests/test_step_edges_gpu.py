@@ -1,6 +1,8 @@
 """Edges of the serving-step operators (squish_b200.ops.step) on the GPU: each test is a call that the
 documentation allows, or a refusal, next to the limits of an operator."""
 import math
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -52,6 +54,28 @@ def test_group_sums_of_opposite_biases_are_ranked_exactly(cuda, B, score, groups
 
 
 # ----------------------------------------------------------------------------- layout
+@pytest.mark.parametrize("B", [3065, 3066, 3069, 3071, 3073])
+def test_layout_sizes_around_48_kb_of_shared_memory(cuda, B):
+    """The first launch of a process (a larger step before it would raise the kernel's limit)."""
+    code = f"""
+import torch
+from squish_b200 import ops
+from tests._step_refs import layout_ref
+B = {B}
+i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+lay = ops.StepLayout(B, B, 2 * B)
+table = [[b] for b in range(B)]
+tab = i32(table)
+ops.step_layout(i32([1] * B), i32([1] * B), tab, i32([]), 4, lay)
+want = layout_ref([1] * B, [1] * B, table, [], 4, 32, B, 2 * B)
+for k, v in want.items():
+    assert getattr(lay, k).tolist() == v, k
+ops.workspace(torch.device("cuda", 0)).check()
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_layout_sequences_that_do_not_fit_keep_their_length(cuda):
     """Without pages, table columns or rows for all of its tokens a sequence rests: kv_len is that of the
     pages it has, last_row -1, its attention tiles padding; the others are as without it."""
