@@ -790,6 +790,7 @@ __global__ void __launch_bounds__(256) prefill_kernel(const AttnParams p) {
   const int b = p.tile_seq[tile];
   const int q0 = p.tile_q0[tile];
   const int qlen = p.q_len[b];
+  if (q0 >= qlen) return;  // whole CTA: a padding tile (step_layout) reads nothing of its sequence
   const int ctx = p.ctx_len[b];
   const int qn = min(PQ, qlen - q0);
   const int pos0 = ctx - qlen + q0;  // absolute position of query row 0

@@ -154,3 +154,27 @@ def test_attention_reads_no_page_that_a_sequence_did_not_get(cuda):
                                 lay.tile_seq.numel(), out, hq, hkv, d, ps, 32, fk, fv, 1 / math.sqrt(d))
     assert (out[1:] == 3).all() and not (out[0] == 3).all()
     assert status(cuda) == 6
+
+
+def test_padding_tiles_do_not_read_the_cache(cuda):
+    """A padding tile names sequence 0: whatever that sequence's table holds, it is not looked at (bf16 KV,
+    which the tensor-core kernel does not serve)."""
+    hq, hkv, d, ps, pages = 4, 2, 64, 16, 4
+    cache, kv = paged(cuda, pages, hkv, ps, d, 0)
+    ops.workspace(cuda).status.zero_()
+    fk, fv = K.KV_FORMATS["bf16"]
+    lay = ops.StepLayout(2, 40, device=cuda)
+    # sequence 0 rests; its entries were given to nobody (10^6 lies outside the pool)
+    tab = torch.tensor([[10**6, 10**6, 10**6], [2, 1, 3]], dtype=torch.int32, device=cuda)
+    ops.step_layout(i32([40, 13], cuda), i32([0, 20], cuda), tab, i32([1, 3, 0], cuda), ps, lay)
+    assert lay.tile_q0.tolist().count(PAD_Q0) == 2 and lay.tile_seq.tolist()[1:] == [0, 0]
+    x = torch.randn(40, hq * d, generator=torch.Generator().manual_seed(1)).to(BF).to(cuda)
+    out = torch.full((40, hq * d), 3.0, dtype=BF, device=cuda)
+    ops.paged_prefill_attention(x, *cache, tab, lay.tile_seq, lay.tile_q0, lay.q_start[:2], i32([0, 20], cuda),
+                                lay.kv_len, lay.tile_seq.numel(), out, hq, hkv, d, ps, 32, fk, fv, 1 / math.sqrt(d))
+    assert status(cuda) == 0
+    assert (out[20:] == 3).all()
+    rows = [t[[2, 1, 3]].transpose(1, 2).reshape(3 * ps, hkv, d) for t in kv]
+    for i in range(20):
+        want, tol = attend(x[i], *rows, 13 + i + 1)
+        assert ((out[i].double().cpu() - want).abs() <= tol).all()
