@@ -14,6 +14,10 @@ import os
 from dataclasses import dataclass, field
 
 
+# Tensors that hold a MoE router's choice bias, under "model.layers.N.mlp."
+ROUTER_BIAS_NAMES = ("gate.e_score_correction_bias", "gate.bias")
+
+
 @dataclass
 class ModelConfig:
     name: str
@@ -39,7 +43,7 @@ class ModelConfig:
     expert_offset: int = 0       # expert parallelism: this rank holds experts
     num_local_experts: int = 0   # [expert_offset, expert_offset + num_local_experts) (0 = all)
     # router (ops.moe_route_scored): scores, expert groups of which the best are open, weight scale; a
-    # per-expert choice bias is the checkpoint tensor mlp.gate.bias
+    # per-expert choice bias is the checkpoint tensor named in ROUTER_BIAS_NAMES
     router_score: str = "softmax"      # "softmax" | "sigmoid"
     router_groups: int = 1
     router_top_groups: int = 0         # open groups (0 = all)

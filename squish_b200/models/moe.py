@@ -81,6 +81,7 @@ class MoELayer:
         from .decoder import _as_q4a
 
         cfg, t = ck.config, ck.tensors
+        bias_name = ck.router_bias_name(layer)
         dev = torch.device(device)
         p = f"model.layers.{layer}.mlp."
         g = ck.quant.group_size
@@ -93,7 +94,7 @@ class MoELayer:
             d = _as_q4a(t[q + "down_proj.weight"], g)
             dn.append(ops.prepare_int4_weight(d.packed, d.scales, d.offsets, d.shape[1], d.group, dev))
         gate_w = t[p + "gate.weight"].data.to(dev, torch.bfloat16).contiguous()
-        bias = t[p + "gate.bias"].data.to(dev, torch.float32).contiguous() if p + "gate.bias" in t else None
+        bias = t[bias_name].data.to(dev, torch.float32).contiguous() if bias_name else None
         return cls(cfg, gate_w, K_.stack_int4_experts(gu), K_.stack_int4_experts(dn), scratch, bias)
 
     def route(self, logits: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor) -> None:

@@ -19,7 +19,7 @@ import torch
 
 from .._ext import native
 from ..ops.kernels import KV_FORMATS
-from .config import ModelConfig, QuantConfig
+from .config import ROUTER_BIAS_NAMES, ModelConfig, QuantConfig
 from .weights import Checkpoint
 
 
@@ -76,6 +76,9 @@ class ReferenceModel:
         self.q: QuantConfig = ck.quant
         cfg = self.cfg
         self.device = torch.device(device)
+        if cfg.is_moe:
+            for i in range(cfg.num_layers):
+                ck.router_bias_name(i)
         self.w = {k: v.dequantize().float().to(self.device) for k, v in ck.tensors.items()}
         self.cos_sin = rope_table(cfg, min(cfg.max_position, 8192)).to(self.device)
         self.fk, self.fv = KV_FORMATS[self.q.kv_dtype]
@@ -156,7 +159,7 @@ class ReferenceModel:
         """(weights, global expert ids) [T, K] of the router of MoE layer ``p``."""
         cfg = self.cfg
         logits = x @ self.w[p + "mlp.gate.weight"].T
-        bias = self.w[p + "mlp.gate.bias"] if p + "mlp.gate.bias" in self.w else None
+        bias = next((self.w[p + "mlp." + n] for n in ROUTER_BIAS_NAMES if p + "mlp." + n in self.w), None)
         if cfg.plain_router and bias is None:
             probs = torch.softmax(logits, dim=-1)
             topv, topi = probs.topk(cfg.num_experts_per_tok, dim=-1)

@@ -19,7 +19,7 @@ from dataclasses import dataclass, field
 import torch
 
 from .._ext import native
-from .config import ModelConfig, QuantConfig
+from .config import ROUTER_BIAS_NAMES, ModelConfig, QuantConfig
 
 
 @dataclass
@@ -67,6 +67,15 @@ class Checkpoint:
 
     def __contains__(self, name: str) -> bool:
         return name in self.tensors
+
+    def router_bias_name(self, layer: int) -> str | None:
+        """The tensor with the choice bias of a MoE layer's router, or None; ValueError where it
+        is not one value per expert."""
+        p = f"model.layers.{layer}.mlp."
+        name = next((p + n for n in ROUTER_BIAS_NAMES if p + n in self.tensors), None)
+        if name is not None and tuple(self.tensors[name].shape) != (self.config.num_experts,):
+            raise ValueError(f"{name} needs one value for each of {self.config.num_experts} experts")
+        return name
 
     def nbytes(self) -> int:
         n = 0

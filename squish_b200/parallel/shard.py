@@ -132,8 +132,9 @@ def shard_checkpoint(ck: Checkpoint, rank: int, tp: int) -> Checkpoint:
             e_loc = cfg.num_experts // tp
             lc.expert_offset = rank * e_loc
             out.tensors[m + "gate.weight"] = t[m + "gate.weight"]  # the router sees every expert
-            if m + "gate.bias" in t:
-                out.tensors[m + "gate.bias"] = t[m + "gate.bias"]
+            bias = ck.router_bias_name(i)
+            if bias:
+                out.tensors[bias] = t[bias]
             for e in range(rank * e_loc, (rank + 1) * e_loc):
                 for n in ("gate_proj", "up_proj", "down_proj"):
                     out.tensors[m + f"experts.{e}.{n}.weight"] = t[m + f"experts.{e}.{n}.weight"]

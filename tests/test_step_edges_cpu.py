@@ -1,0 +1,41 @@
+"""Edges of the scored router in the models, without a GPU."""
+import dataclasses
+
+import pytest
+import torch
+
+from squish_b200.models.reference import ReferenceModel
+
+from .test_step_ops_cpu import _scored_moe
+
+P = "model.layers.0.mlp."
+
+
+def rename(ck, new):
+    """The checkpoint with its router biases under another name (None: without them)."""
+    for i in range(ck.config.num_layers):
+        t = ck.tensors.pop(f"model.layers.{i}.mlp.gate.bias")
+        if new:
+            ck.tensors[f"model.layers.{i}.mlp.{new}"] = t
+    return ck
+
+
+# ----------------------------------------------------------------------------- config and tensor names
+def test_router_bias_under_its_published_name():
+    from squish_b200.parallel.shard import shard_checkpoint
+
+    x = torch.randn(9, 256, generator=torch.Generator().manual_seed(1))
+    want = ReferenceModel(_scored_moe()[2]).route("model.layers.0.", x)
+    none = ReferenceModel(rename(_scored_moe()[2], None)).route("model.layers.0.", x)
+    assert not torch.equal(none[1], want[1])  # (the bias matters)
+    ck = rename(_scored_moe()[2], "gate.e_score_correction_bias")
+    got = ReferenceModel(ck).route("model.layers.0.", x)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert P + "gate.e_score_correction_bias" in shard_checkpoint(ck, 1, 2).tensors
+
+
+def test_a_router_bias_of_another_length_is_refused():
+    ck = _scored_moe()[2]
+    ck.tensors[P + "gate.bias"] = dataclasses.replace(ck.tensors[P + "gate.bias"], shape=(3,), data=torch.zeros(3))
+    with pytest.raises(ValueError, match="one value for each of 16 experts"):
+        ReferenceModel(ck)
