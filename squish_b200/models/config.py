@@ -49,6 +49,7 @@ class ModelConfig:
     router_top_groups: int = 0         # open groups (0 = all)
     router_group_score: str = "max"    # a group's rank: its best choice score, or "top2": the sum of two
     router_scale: float = 1.0
+    router_bias: bool = False          # every MoE layer of the checkpoint has to bring a choice bias
     rope_scaling: dict | None = None
     bos_token_id: int = 1
     eos_token_id: int = 2
@@ -198,8 +199,9 @@ def from_hf_config(path: str) -> ModelConfig:
         router_score=d.get("scoring_func") or "softmax",
         router_groups=d.get("n_group") or 1,
         router_top_groups=d.get("topk_group") or 0,
-        router_group_score="top2" if d.get("topk_method") == "noaux_tc" else "max",
+        router_group_score=d.get("router_group_score") or ("top2" if d.get("topk_method") == "noaux_tc" else "max"),
         router_scale=d.get("routed_scaling_factor") or 1.0,
+        router_bias=d.get("topk_method") == "noaux_tc",
         rope_scaling=d.get("rope_scaling"),
         bos_token_id=d.get("bos_token_id", 1) or 1,
         eos_token_id=eos,
@@ -233,10 +235,11 @@ def to_hf_config(cfg: ModelConfig) -> dict:
         d.update(num_experts=cfg.num_experts, num_experts_per_tok=cfg.num_experts_per_tok,
                  moe_intermediate_size=cfg.moe_intermediate_size, norm_topk_prob=cfg.norm_topk_prob,
                  decoder_sparse_step=1, mlp_only_layers=[])
-        if not cfg.plain_router:
+        if not cfg.plain_router or cfg.router_bias:
             d.update(scoring_func=cfg.router_score, n_group=cfg.router_groups,
-                     topk_group=cfg.router_top_groups or cfg.router_groups, routed_scaling_factor=cfg.router_scale)
-            if cfg.router_group_score == "top2":
+                     topk_group=cfg.router_top_groups or cfg.router_groups, routed_scaling_factor=cfg.router_scale,
+                     router_group_score=cfg.router_group_score)
+            if cfg.router_bias:
                 d["topk_method"] = "noaux_tc"
     if cfg.rope_scaling:
         d["rope_scaling"] = cfg.rope_scaling

@@ -69,10 +69,12 @@ class Checkpoint:
         return name in self.tensors
 
     def router_bias_name(self, layer: int) -> str | None:
-        """The tensor with the choice bias of a MoE layer's router, or None; ValueError where it
-        is not one value per expert."""
+        """The tensor with the choice bias of a MoE layer's router, or None; ValueError where the config
+        asks for one and there is none, or it is not one value per expert."""
         p = f"model.layers.{layer}.mlp."
         name = next((p + n for n in ROUTER_BIAS_NAMES if p + n in self.tensors), None)
+        if name is None and self.config.router_bias:
+            raise ValueError(f"the config's router has a choice bias, but the checkpoint has no {p}{ROUTER_BIAS_NAMES[0]}")
         if name is not None and tuple(self.tensors[name].shape) != (self.config.num_experts,):
             raise ValueError(f"{name} needs one value for each of {self.config.num_experts} experts")
         return name

@@ -1,9 +1,11 @@
 """Edges of the scored router in the models, without a GPU."""
 import dataclasses
+import json
 
 import pytest
 import torch
 
+from squish_b200.models.config import from_hf_config, get_preset, to_hf_config
 from squish_b200.models.reference import ReferenceModel
 
 from .test_step_ops_cpu import _scored_moe
@@ -21,6 +23,16 @@ def rename(ck, new):
 
 
 # ----------------------------------------------------------------------------- config and tensor names
+@pytest.mark.parametrize("kw", [dict(router_group_score="top2", router_groups=4), dict(router_bias=True),
+                                dict(router_score="sigmoid", router_bias=True, router_groups=2)])
+def test_router_fields_survive_a_config_file(tmp_path, kw):
+    cfg = dataclasses.replace(get_preset("tiny-moe")[0], **kw)
+    (tmp_path / "config.json").write_text(json.dumps(to_hf_config(cfg)))
+    back = from_hf_config(str(tmp_path))
+    for f in ("router_score", "router_groups", "router_group_score", "router_scale", "router_bias"):
+        assert getattr(back, f) == getattr(cfg, f), f
+
+
 def test_router_bias_under_its_published_name():
     from squish_b200.parallel.shard import shard_checkpoint
 
@@ -32,6 +44,17 @@ def test_router_bias_under_its_published_name():
     got = ReferenceModel(ck).route("model.layers.0.", x)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert P + "gate.e_score_correction_bias" in shard_checkpoint(ck, 1, 2).tensors
+
+
+def test_a_missing_router_bias_is_refused():
+    from squish_b200.models.moe import MoELayer
+    from squish_b200.parallel.shard import shard_checkpoint
+
+    ck = rename(_scored_moe()[2], None)
+    ck.config = dataclasses.replace(ck.config, router_bias=True)
+    for load in (ReferenceModel, lambda c: shard_checkpoint(c, 0, 2), lambda c: MoELayer.from_checkpoint(c, 0, "cpu")):
+        with pytest.raises(ValueError, match="no model.layers.0.mlp.gate.e_score_correction_bias"):
+            load(ck)
 
 
 def test_a_router_bias_of_another_length_is_refused():
