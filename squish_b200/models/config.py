@@ -63,6 +63,20 @@ class ModelConfig:
         """Softmax over all experts, top-k, no scale: the routing of moe_route."""
         return self.router_score == "softmax" and self.router_groups == 1 and self.router_scale == 1.0
 
+    def check_router(self) -> None:
+        """ValueError for router fields that name no rule, or that leave fewer open experts than picks."""
+        if not self.is_moe or self.plain_router:
+            return
+        if self.router_score not in ("softmax", "sigmoid"):
+            raise ValueError(f"router scores are 'softmax' or 'sigmoid', not {self.router_score!r}")
+        if self.router_group_score not in ("max", "top2"):
+            raise ValueError(f"a router's group score is 'max' or 'top2', not {self.router_group_score!r}")
+        g, top = self.router_groups, self.router_top_groups or self.router_groups
+        if g < 1 or self.num_experts % g or not 1 <= top <= g:
+            raise ValueError(f"{self.num_experts} experts do not split into {g} groups of which {top} are open")
+        if self.num_experts_per_tok > self.num_experts // g * top:
+            raise ValueError(f"{self.num_experts_per_tok} picks from {self.num_experts // g * top} open experts")
+
     @property
     def q_size(self) -> int:
         return self.num_heads * self.head_dim
@@ -176,7 +190,11 @@ def from_hf_config(path: str) -> ModelConfig:
     eos = d.get("eos_token_id", 2)
     if isinstance(eos, list):
         eos = eos[0]
-    return ModelConfig(
+    method = d.get("topk_method") if d.get("num_experts") else None
+    if method not in (None, "greedy", "group_limited_greedy", "noaux_tc"):
+        raise ValueError(f"unsupported topk_method {method!r}")
+    grouped = method != "greedy"  # (greedy: the best of all experts, whatever n_group says)
+    cfg = ModelConfig(
         name=d.get("_name_or_path", os.path.basename(os.path.dirname(p))) or mt,
         arch=arch,
         vocab_size=d["vocab_size"],
@@ -197,15 +215,17 @@ def from_hf_config(path: str) -> ModelConfig:
         moe_intermediate_size=d.get("moe_intermediate_size", 0) or 0,
         norm_topk_prob=d.get("norm_topk_prob", True),
         router_score=d.get("scoring_func") or "softmax",
-        router_groups=d.get("n_group") or 1,
-        router_top_groups=d.get("topk_group") or 0,
-        router_group_score=d.get("router_group_score") or ("top2" if d.get("topk_method") == "noaux_tc" else "max"),
+        router_groups=(d.get("n_group") or 1) if grouped else 1,
+        router_top_groups=(d.get("topk_group") or 0) if grouped else 0,
+        router_group_score=d.get("router_group_score") or ("top2" if method == "noaux_tc" else "max"),
         router_scale=d.get("routed_scaling_factor") or 1.0,
-        router_bias=d.get("topk_method") == "noaux_tc",
+        router_bias=method == "noaux_tc",
         rope_scaling=d.get("rope_scaling"),
         bos_token_id=d.get("bos_token_id", 1) or 1,
         eos_token_id=eos,
     )
+    cfg.check_router()
+    return cfg
 
 
 def to_hf_config(cfg: ModelConfig) -> dict:

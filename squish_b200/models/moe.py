@@ -81,6 +81,7 @@ class MoELayer:
         from .decoder import _as_q4a
 
         cfg, t = ck.config, ck.tensors
+        cfg.check_router()
         bias_name = ck.router_bias_name(layer)
         dev = torch.device(device)
         p = f"model.layers.{layer}.mlp."

@@ -77,6 +77,7 @@ class ReferenceModel:
         cfg = self.cfg
         self.device = torch.device(device)
         if cfg.is_moe:
+            cfg.check_router()
             for i in range(cfg.num_layers):
                 ck.router_bias_name(i)
         self.w = {k: v.dequantize().float().to(self.device) for k, v in ck.tensors.items()}

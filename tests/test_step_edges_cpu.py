@@ -13,6 +13,13 @@ from .test_step_ops_cpu import _scored_moe
 P = "model.layers.0.mlp."
 
 
+def read_config(tmp_path, **fields):
+    d = to_hf_config(get_preset("tiny-moe")[0])
+    d.update(fields)
+    (tmp_path / "config.json").write_text(json.dumps(d))
+    return from_hf_config(str(tmp_path))
+
+
 def rename(ck, new):
     """The checkpoint with its router biases under another name (None: without them)."""
     for i in range(ck.config.num_layers):
@@ -23,6 +30,24 @@ def rename(ck, new):
 
 
 # ----------------------------------------------------------------------------- config and tensor names
+def test_published_router_fields(tmp_path):
+    c = read_config(tmp_path, scoring_func="sigmoid", n_group=4, topk_group=2, topk_method="noaux_tc",
+                    routed_scaling_factor=2.5)
+    assert (c.router_score, c.router_groups, c.router_top_groups, c.router_group_score, c.router_scale,
+            c.router_bias) == ("sigmoid", 4, 2, "top2", 2.5, True)
+    c = read_config(tmp_path, n_group=4, topk_group=2, topk_method="group_limited_greedy")
+    assert (c.router_groups, c.router_top_groups, c.router_group_score, c.router_bias) == (4, 2, "max", False)
+    # greedy: the best of all experts, whatever the groups say
+    c = read_config(tmp_path, n_group=4, topk_group=2, topk_method="greedy")
+    assert c.router_groups == 1 and c.plain_router
+    for bad, msg in [(dict(topk_method="hash"), "topk_method 'hash'"), (dict(scoring_func="relu"), "router scores"),
+                     (dict(n_group=3), "do not split"), (dict(n_group=4, topk_group=5), "do not split"),
+                     (dict(n_group=8, topk_group=1), "4 picks from 2 open"),
+                     (dict(n_group=4, router_group_score="mean"), "group score")]:
+        with pytest.raises(ValueError, match=msg):
+            read_config(tmp_path, **bad)
+
+
 @pytest.mark.parametrize("kw", [dict(router_group_score="top2", router_groups=4), dict(router_bias=True),
                                 dict(router_score="sigmoid", router_bias=True, router_groups=2)])
 def test_router_fields_survive_a_config_file(tmp_path, kw):
