@@ -165,20 +165,44 @@ class ReferenceModel:
             probs = torch.softmax(logits, dim=-1)
             topv, topi = probs.topk(cfg.num_experts_per_tok, dim=-1)
         else:
-            probs = torch.sigmoid(logits) if cfg.router_score == "sigmoid" else torch.softmax(logits, dim=-1)
-            choice = probs if bias is None else probs + bias
-            G = cfg.router_groups
-            if G > 1:
-                grp = choice.view(choice.shape[0], G, -1)
-                n = min(2, grp.shape[-1]) if cfg.router_group_score == "top2" else 1
-                best = grp.topk(n, dim=-1).values.sum(-1).topk(cfg.router_top_groups or G, dim=-1).indices
-                closed = torch.ones_like(grp[..., 0], dtype=torch.bool).scatter_(1, best, False)
-                choice = choice.masked_fill(closed.repeat_interleave(grp.shape[-1], dim=1), float("-inf"))
-            topi = choice.topk(cfg.num_experts_per_tok, dim=-1).indices
-            topv = probs.gather(-1, topi)
+            topv, topi = self._route_scored(logits.double(), bias)
+            return topv.float(), topi
         if cfg.norm_topk_prob:
             topv = topv / topv.sum(-1, keepdim=True)
-        return (topv if cfg.router_scale == 1.0 else topv * cfg.router_scale), topi
+        return topv, topi
+
+    def _route_scored(self, x: torch.Tensor, bias: torch.Tensor | None):
+        """The rules of ops.moe_route_scored in 64 bits: a NaN logit counts as -inf, equal values go to the
+        lower index, without a bias the choice follows the logits (both scores are monotone in them)."""
+        cfg = self.cfg
+        neg = float("-inf")
+        x = torch.where(x.isnan(), neg, x)
+        if cfg.router_score == "sigmoid":
+            probs = torch.sigmoid(x)
+        else:
+            m = x.amax(-1, keepdim=True)
+            e = torch.where(x == m, 1.0, torch.exp(x - m)).masked_fill(x == neg, 0.0)
+            z = e.sum(-1, keepdim=True)
+            probs = e / torch.where(z > 0, z, 1.0)
+        choice = x if bias is None else probs + bias.double()
+        choice = torch.where(choice.isnan(), neg, choice)
+        G, E = cfg.router_groups, choice.shape[1]
+        order = choice.sort(dim=-1, descending=True, stable=True).indices
+        if G > 1:
+            two = cfg.router_group_score == "top2" and E // G > 1
+            rank = probs if two and bias is None else choice
+            best = rank.view(-1, G, E // G).topk(2 if two else 1, dim=-1).values.sum(-1)
+            best = torch.where(best.isnan(), neg, best)
+            opened = best.sort(dim=-1, descending=True, stable=True).indices[:, :cfg.router_top_groups or G]
+            is_open = torch.zeros_like(best, dtype=torch.bool).scatter_(1, opened, True).repeat_interleave(E // G, 1)
+            # open experts first, each kind in its order (a closed one never replaces an open one of -inf)
+            order = order.gather(1, (~is_open.gather(1, order)).to(torch.int8).sort(dim=-1, stable=True).indices)
+        topi = order[:, :cfg.num_experts_per_tok]
+        topv = probs.gather(-1, topi)
+        if cfg.norm_topk_prob:
+            total = topv.sum(-1, keepdim=True)
+            topv = topv / torch.where(total > 0, total, 1.0)
+        return topv * cfg.router_scale, topi
 
     def expert(self, p: str, e: int, xr: torch.Tensor) -> torch.Tensor:
         """Expert ``e`` (global id) of MoE layer ``p`` on one row."""

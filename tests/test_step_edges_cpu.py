@@ -2,12 +2,14 @@
 import dataclasses
 import json
 
+import numpy as np
 import pytest
 import torch
 
 from squish_b200.models.config import from_hf_config, get_preset, to_hf_config
 from squish_b200.models.reference import ReferenceModel
 
+from ._step_refs import route_ref
 from .test_step_ops_cpu import _scored_moe
 
 P = "model.layers.0.mlp."
@@ -87,3 +89,41 @@ def test_a_router_bias_of_another_length_is_refused():
     ck.tensors[P + "gate.bias"] = dataclasses.replace(ck.tensors[P + "gate.bias"], shape=(3,), data=torch.zeros(3))
     with pytest.raises(ValueError, match="one value for each of 16 experts"):
         ReferenceModel(ck)
+
+
+# ----------------------------------------------------------------------------- the CPU model's choice
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("kw", [
+    dict(router_score="sigmoid", router_groups=1, router_top_groups=0, router_group_score="max"),
+    dict(router_score="sigmoid", router_groups=4, router_top_groups=2, router_group_score="top2"),
+    dict(router_score="softmax", router_groups=4, router_top_groups=2, router_group_score="max"),
+    dict(router_score="softmax", router_groups=8, router_top_groups=5, router_group_score="top2"),
+    dict(router_score="softmax", router_groups=2, router_top_groups=1, norm_topk_prob=False),
+])
+def test_cpu_router_decides_like_the_kernel(kw, biased):
+    """Equal scores go to the lower index, saturated ones are told apart, masked experts in an open group
+    come before closed ones: the rules of ops.moe_route_scored."""
+    ck = _scored_moe()[2]
+    ck.config = c = dataclasses.replace(ck.config, **kw)
+    ref = ReferenceModel(ck)
+    E = c.num_experts
+    g = torch.Generator().manual_seed(3)
+    ref.w.pop(P + "gate.bias")
+    if biased:
+        b = torch.randint(0, 2, (E,), generator=g).float() * 0.25
+        b[8:] = -float("inf")
+        b[12] = 0.0  # the last groups: one expert left, or none
+        ref.w[P + "gate.bias"] = b
+    ref.w[P + "gate.weight"] = torch.eye(E, c.hidden_size)
+    x = torch.zeros(40, c.hidden_size)
+    x[:, :E] = torch.randint(-2, 3, (40, E), generator=g).float()
+    x[0, :E] = 0.0
+    x[1, :E] = torch.linspace(18, 30, E)     # 1 in 32 bits
+    x[2, :E] = torch.linspace(-150, -120, E)  # 0 in 32 bits
+    w, ids = ref.route("model.layers.0.", x)
+    want_i, want_w = route_ref(x[:, :E], c.num_experts_per_tok, c.router_score, ref.w.get(P + "gate.bias"),
+                               c.router_groups, c.router_top_groups or None, c.router_group_score, c.norm_topk_prob,
+                               c.router_scale)
+    assert np.array_equal(ids.numpy(), want_i)
+    # (64-bit weights, rounded to 32 bits once)
+    np.testing.assert_allclose(w.double().numpy(), want_w, rtol=2.0**-23, atol=2.0**-149)
