@@ -2,7 +2,7 @@
 
 Per shard: load tensors (on the GPU when one is present, where the INT4 quantizer runs as a
 CUDA kernel), quantize every 2-D projection weight, pass embeddings, norms, biases and MoE
-routers through as fp16, write the tensor files, then commit ``manifest.json`` and
+routers through as fp16 (a router's choice bias as float32), write the tensor files, then commit ``manifest.json`` and
 ``_compress_progress.json`` (completed shards) before moving on — the reference's
 streaming converter contract (squish/convert.py:610-935). Re-running after an interruption
 skips completed shards. ``delete_source`` removes a raw shard only after its output and

@@ -40,6 +40,7 @@ from pathlib import Path
 import numpy as np
 import torch
 
+from ..models.config import ROUTER_BIAS_NAMES
 from ..models.weights import Checkpoint, QTensor
 
 SUFFIXES = ("__pt_df11", "__vq_idx", "__vq_cb", "__vq_res", "__vq_rescb", "__vq_cols", "__vq_meta", "__lv_nf4", "__nf4",
@@ -210,7 +211,8 @@ def read_npy_dir(path: str | Path, config, quant) -> Checkpoint:
 
 def tensor_files(name: str, t: QTensor, df11: bool = False) -> dict[str, np.ndarray]:
     """The npy-dir files of one tensor (suffix -> array); ``df11`` stores dense tensors as
-    lossless bf16 ``__pt_df11`` instead of float16 ``__pt``."""
+    lossless bf16 ``__pt_df11`` instead of float16 ``__pt``. A router's choice bias stays float32: it
+    decides between scores that 16 bits do not tell apart."""
     k = safe_key(name)
     out = {f"{k}__shape": np.asarray(t.shape, dtype=np.int64)}
 
@@ -248,6 +250,8 @@ def tensor_files(name: str, t: QTensor, df11: bool = False) -> dict[str, np.ndar
             out[f"{k}__{kk}"] = np_(v, np.float32)
     elif t.kind == "aqlm":
         out.update({f"{k}__aqlm_idx": np_(t.packed, np.uint16), f"{k}__aqlm_cb": np_(t.scales, np.float32)})
+    elif t.kind == "dense" and name.endswith(tuple(f".mlp.{n}" for n in ROUTER_BIAS_NAMES)):
+        out[f"{k}__pt"] = np_(t.data.float(), np.float32)
     elif t.kind == "dense" and df11:
         from .entropy import df11_encode
 

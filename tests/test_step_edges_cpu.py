@@ -91,6 +91,30 @@ def test_a_router_bias_of_another_length_is_refused():
         ReferenceModel(ck)
 
 
+@pytest.mark.parametrize("name", ["gate.bias", "gate.e_score_correction_bias"])
+@pytest.mark.parametrize("df11", [False, True])
+def test_router_bias_keeps_its_bits_through_compress(tmp_path, name, df11):
+    """A choice bias near 8 whose values differ by less than a float16 step there."""
+    from safetensors.torch import save_file
+
+    from squish_b200.io.convert import compress, load_checkpoint
+
+    ck = rename(_scored_moe()[2], name)
+    cfg = ck.config
+    src, out = tmp_path / "src", tmp_path / "out"
+    src.mkdir()
+    (src / "config.json").write_text(json.dumps(to_hf_config(cfg)))
+    bias = 8.0 + torch.randperm(cfg.num_experts, generator=torch.Generator().manual_seed(0)).float() * 2.0**-16
+    tensors = {k: v.dequantize().to(torch.bfloat16).contiguous() for k, v in ck.tensors.items()}
+    for i in range(cfg.num_layers):
+        tensors[f"model.layers.{i}.mlp.{name}"] = bias.clone()
+    save_file(tensors, str(src / "model.safetensors"))
+    compress(str(src), str(out), device="cpu", df11=df11, log=lambda *_: None)
+    back = load_checkpoint(str(out), "cpu")[0]
+    for i in range(cfg.num_layers):
+        assert torch.equal(back[f"model.layers.{i}.mlp.{name}"].data.float(), bias)
+
+
 # ----------------------------------------------------------------------------- the CPU model's choice
 @pytest.mark.parametrize("biased", [False, True])
 @pytest.mark.parametrize("kw", [
