@@ -77,15 +77,20 @@ void step_layout(torch::Tensor ctx, torch::Tensor q, torch::Tensor tables, torch
   p.tile = (int)tile;
   p.token_cap = (int)cap;
   p.tile_cap = (int)tcap;
-  // (blocks read the lengths while others already write the results)
+  // (blocks read the lengths and the free list while others already write the results and the tables)
+  auto share = [](const torch::Tensor& t, int64_t n, const torch::Tensor& u, int64_t m) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr()), b = reinterpret_cast<uintptr_t>(u.data_ptr());
+    return n > 0 && m > 0 && a < b + 4 * m && b < a + 4 * n;
+  };
+  const int64_t table_n = tables.size(1) > 0 ? (B - 1) * tables.stride(0) + tables.size(1) : 0;
   auto apart = [&](const torch::Tensor& t, const char* name, int64_t n) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr()), b = reinterpret_cast<uintptr_t>(out.data_ptr());
-    TORCH_CHECK(n == 0 || a >= b + 4 * out.numel() || b >= a + 4 * n, name, " is part of the step layout it makes");
+    TORCH_CHECK(!share(t, n, out, out.numel()), name, " is part of the step layout it makes");
+    TORCH_CHECK(!share(t, n, tables, table_n), name, " is part of block_tables");
   };
   apart(ctx, "ctx_len", B);
   apart(q, "q_len", B);
   apart(free_pages, "free_pages", free_pages.numel());
-  apart(tables, "block_tables", B > 0 ? (B - 1) * tables.stride(0) + tables.size(1) : 0);
+  TORCH_CHECK(!share(tables, table_n, out, out.numel()), "block_tables is part of the step layout it makes");
   // one buffer, its rows in this order, each padded to a multiple of four (ops.step.StepLayout)
   auto pad = [](int64_t n) { return (n + 3) / 4 * 4; };
   int* at = arr<int>(out, "the step layout", I32, dev,

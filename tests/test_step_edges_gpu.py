@@ -110,6 +110,23 @@ def test_layout_sequences_that_do_not_fit_keep_their_length(cuda):
     assert lay.kv_len.tolist() == [2] * 4 and lay.last_row.tolist() == [-1] * 4 and status(cuda) == 6
 
 
+def test_layout_inputs_inside_the_tables_are_refused(cuda):
+    """(other blocks write the tables while the lengths and the free list are read)"""
+    lay = ops.StepLayout(2, 8, device=cuda)
+    tab = torch.zeros(2, 4, dtype=torch.int32, device=cuda)
+    ok = dict(c=i32([0, 0], cuda), q=i32([1, 1], cuda), f=i32([1, 2, 3], cuda))
+    for k, name in (("c", "ctx_len"), ("q", "q_len"), ("f", "free_pages")):
+        a = {**ok, k: tab[1, 1:3]}
+        with pytest.raises(RuntimeError, match=name + " is part of block_tables"):
+            ops.step_layout(a["c"], a["q"], tab, a["f"], 4, lay)
+    with pytest.raises(RuntimeError, match="block_tables is part of the step layout"):
+        ops.step_layout(ok["c"], ok["q"], lay.buf[:8].view(2, 4), ok["f"], 4, lay)
+    arena = torch.zeros(16, dtype=torch.int32, device=cuda)  # neighbours in one buffer are allowed
+    arena[10:12] = 1
+    ops.step_layout(arena[8:10], arena[10:12], arena[:8].view(2, 4), arena[12:16], 4, lay)
+    assert lay.kv_len.tolist() == [1, 1] and status(cuda) == 0
+
+
 def paged(cuda, pages, hkv, ps, d, seed):
     """bf16 KV pages with values, and [pages * ps, hkv, d] views of keys and values."""
     g = torch.Generator().manual_seed(seed)
