@@ -195,3 +195,35 @@ def test_padding_tiles_do_not_read_the_cache(cuda):
     for i in range(20):
         want, tol = attend(x[i], *rows, 13 + i + 1)
         assert ((out[i].double().cpu() - want).abs() <= tol).all()
+
+
+# ----------------------------------------------------------------------------- in the model
+@pytest.mark.parametrize("graphs", [False, True])
+def test_scored_router_decode_steps_follow_the_cpu_model(cuda, graphs):
+    """Each decode step's logits, launched eagerly and from captured graphs, against the CPU model fed the
+    tokens that the engine drew."""
+    from squish_b200.engine.engine import EngineConfig, LLMEngine
+    from squish_b200.engine.sampling import SamplingParams
+    from squish_b200.models.reference import ReferenceModel
+
+    from .test_step_ops_cpu import _scored_moe
+
+    cfg, _, ck = _scored_moe()
+    ref = ReferenceModel(ck)
+    prompt = np.random.default_rng(7).integers(0, cfg.vocab_size, 21).tolist()
+    eng = LLMEngine.from_checkpoint(ck, cuda, EngineConfig(max_num_seqs=4, max_num_batched_tokens=64,
+                                                           max_model_len=256, num_pages=64, cuda_graphs=graphs))
+    rid = eng.add_request(prompt, SamplingParams(max_tokens=6, ignore_eos=True))
+    cache = ref.new_cache()
+    want = ref.forward(prompt, cache, 0)[-1]
+    n = 0
+    while eng.has_unfinished():
+        eng.step()
+        out = eng.requests[rid].output
+        assert len(out) == n + 1
+        got = eng.runner.logits[0].float().cpu()
+        assert torch.nn.functional.cosine_similarity(got, want, dim=0) > 0.99, n
+        n += 1
+        want = ref.forward([out[-1]], cache, len(prompt) + n - 1)[-1]
+    assert n == 6
+    eng.runner.ws.check()
