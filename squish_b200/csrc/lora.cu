@@ -418,7 +418,7 @@ __device__ __forceinline__ uint8_t* align1k(uint8_t* p) {
 // It is bound by bytes, so what it takes is few instructions per byte and enough bytes in flight. 8185
 // rows, K 4096, N 6144, rank up to 64 (268 MB, 42 us at the copy rate): 240 us with mma.sync fragments
 // loaded from global memory, 72 us with the same behind the ring (bound by instruction issue), 60 us
-// this way (4.5 TB/s). 2048 rows, K 3584, N 37888 with the epilogue (254 MB, 39 us): 151, 62, 55 us.
+// this way (4.5 TB/s). 2048 rows, K 3584, N 37888 with the epilogue (254 MB, 39 us): 151, 62, 56 to 60 us.
 // A row's share of a unit is what the memory sees: 64-byte pieces gave 3.3 TB/s in the expand, 128
 // bytes 4.3, 256 bytes 4.7. One CTA of 16 warps per SM instead of two of 8 was slower (66 us), with five
 // stages and each product one unit ahead too (2048 rows, N 37888, rank 16, 16 adapters: 100 against 73 us):
@@ -897,6 +897,8 @@ cudaError_t lora_add_launch(const LoraParams& p, int num_sms, cudaStream_t s) {
   // CTAs per tile (K split over them): more while few tiles leave SMs idle. Measured with 2, 4, 8, tiles
   // of 128 rows: 33 tiles at most, K 3584: 64, 60, 58 us; 82 tiles, K 4096: 65, 61, 65 us; 72 tiles, K
   // 2048: 40, 38, 45 us. Tiles of 16 rows: 1 row 9.4, 7.1, 6.0 us; 37 tiles at most 10.5, 8.0, 8.0 us.
+  // (The number of tiles is known on the device only; its bound grows with the pool's slots, so a large
+  // pool of which a step uses a few gets fewer CTAs than it could: see ops.LoraPool for what that costs.)
   int C = 8;
   while (C > 1 && p.max_tiles * C > (p.tm == 16 ? 4 : 3) * num_sms) C >>= 1;
   switch (p.R) {

@@ -15,9 +15,10 @@
 // Group scores are compared in fp32; where an open and a closed group lie within their own error
 // bounds the same warp ranks the groups again in fp64. So the ids are those of the exact scores.
 //
-// What bounds a large step is instruction issue (some 900 instructions per token; 16384 tokens, 256
-// experts in 8 groups, top 8, bf16: 23 us for 9.4 MB): scores and group sums 10 us of it, the short list
-// 1, exact scores 1.4, picks 2.3, weights 3, and 4 that the few rows ranked again keep the last wave.
+// What bounds a large step is instructions and their latency (16384 tokens, 256 experts in 8 groups, top
+// 8, bf16: 23 us for 9.4 MB; 1114 warp instructions per token, which issue in 69 % of the cycles, the rest
+// are fixed latencies and shuffles that wait for one another): scores and group sums 10 us of it, the short
+// list 1, exact scores 1.4, picks 2.3, weights 3, and 4 that the few rows ranked again keep the last wave.
 // Picking all 8 from 32 * EPL values, and every close row again in fp64, took 41 us.
 #include "kernels.h"
 #include "launch.cuh"

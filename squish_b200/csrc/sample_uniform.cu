@@ -17,16 +17,19 @@
 // share an SM. Two values of a 32-bit word become two byte offsets with three integer operations;
 // a word with another value takes the checked path, and a row with a finite value outside (none
 // comes out of a model, but the format allows it) is done by one CTA in four windows of the whole
-// key space. What bounds a full batch is the shared-memory atomics: one per token, 8 bytes of
-// logits per atomic pair, so the row is loaded in 16-byte groups, four in flight per thread.
+// key space. Counting costs one shared-memory atomic per token (2 bytes of logits), and the row is
+// loaded in 16-byte groups, four in flight per thread.
 //
 // A cluster of C CTAs shares a row when there are few rows: each counts a slice and owns 1/C of the
 // bins (summed over the peers' shared memory); three exchanges through shared memory (masses, kept
 // masses, the drawn value) make the draw, and a fourth keeps the memory alive.
 //
 // Measured (V 152064, temperature only): 1 row 16 us (a chain of five cluster exchanges and as many
-// block sums in fp64, 27000 clocks), 64 rows 23 us, 256 rows 52 us (78 MB: 12 us at the copy rate; 15 us a
-// row on its SM are the atomics, at 2.8 clocks per warp). With one exponential per token, serial walks
+// block sums in fp64, 27000 clocks), 64 rows 23 us, 256 rows 52 us (78 MB: 12 us at the copy rate). The
+// atomics are 7 us of a row on its SM (4752 of its warps', 2.8 clocks each), 14 us for the two rows that
+// share one; in the rest the warps wait, first of all for loads (256 rows with mixed filters and masks, 63
+// us: an instruction issues in 42 % of the cycles, loads are the largest stall, then fixed latencies and
+// barriers), with 256 rows on 148 SMs leaving 40 of them one row. With one exponential per token, serial walks
 // over a thread's bins and counters read in the owner's order it was 34, 78 and 122 us.
 #include <cooperative_groups.h>
 
@@ -903,7 +906,7 @@ cudaError_t sample_uniform_launch(const SampleUniformParams& p, int num_sms, cud
   // CTA is as fast or faster at any batch (1 row of 32000: 13.2 us against 13.9, 13.1, 13.9 with 2, 4, 8;
   // 64 rows: 13.7 against 14.3, 20.3, 42.2). Of 152064 values, us with 1, 2, 4, 8 CTAs: 1 row 23, 19, 17,
   // 16; 8 rows 30, 23, 19, 17; 16 rows 30, 23, 18, 20; 64 rows 30, 23, 26, 47; 100 rows 31, 42, 43, 75 (two
-  // CTAs of two do not fit an SM).
+  // CTAs of two do not fit an SM). Where between the two sizes the change pays most was not measured.
   int c = 1;
   if (p.V > 65536) c = 16 * p.B <= num_sms ? 8 : 8 * p.B <= num_sms ? 4 : 2 * p.B <= num_sms ? 2 : 1;
   switch (c) {

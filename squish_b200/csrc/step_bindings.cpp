@@ -1,6 +1,6 @@
 // step_bindings.cpp — Python bindings of the serving-step operators (step_ops.h). Arguments are
 // checked for device, dtype, shape and layout before the first CUDA call; every call launches on
-// the current stream of its tensors' device and allocates nothing.
+// the current stream of its tensors' device and allocates nothing but lora_add's h (above 512 rows).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

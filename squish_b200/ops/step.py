@@ -138,7 +138,8 @@ def moe_route_scored(logits: torch.Tensor, top_k: int, ids: torch.Tensor, weight
 def fuse_lora(parts: list[tuple[torch.Tensor, torch.Tensor] | None], sizes: list[int], k: int | None = None,
               interleave: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """One (A [r, K], B [N, r]) pair for a fused projection whose output rows are the parts' rows
-    one after another (``sizes`` of them): the ranks add up and B is block-diagonal. ``interleave``:
+    one after another (``sizes`` of them): the ranks add up (to 128 at most for a :class:`LoraPool`: q, k
+    and v of rank 42) and B is block-diagonal. ``interleave``:
     two parts of equal size, gate and up, in [gate 64 | up 64] row blocks (the layout of the fused
     gate_up weight, sizes padded to a multiple of 64). A part may be None (no adapter there)."""
     if len(parts) != len(sizes):
@@ -171,7 +172,12 @@ def fuse_lora(parts: list[tuple[torch.Tensor, torch.Tensor] | None], sizes: list
 class LoraPool:
     """Adapters of one projection [N, K], resident on the device: ``slots`` of them, each A [r, K],
     B [N, r] (r <= ``max_rank`` <= 128) and a scale, in bf16, zero-padded to the pool's rank. The
-    same slot numbers name a request's adapter in every projection's pool."""
+    same slot numbers name a request's adapter in every projection's pool.
+
+    :func:`lora_add` picks its launch for the most tiles that the rows may make, one per slot, so a
+    pool much larger than what a step uses costs time (B200, 5 adapters in a pool of 16 / 256 / 1024 slots,
+    us: 512 rows, 3584 x 4608, rank 16 8.6 / 12 / 19, 3584 x 37888 with SiLU*up 32 / 85 / 164; 2048 rows 18 /
+    27 / 28 and 58 / 68 / 68; 64 rows over 16 adapters, 3584 x 4608 6.5 in each)."""
 
     def __init__(self, slots: int, k: int, n: int, max_rank: int, device="cuda"):
         if slots < 1 or slots > 1024:
@@ -222,7 +228,8 @@ class LoraPlan:
     def __init__(self, rows: int, slots: int, device):
         # tiles of 16 rows while adapters have few rows each, of 128 for prefill: a tile reads its
         # adapter once, so wider tiles re-read less (from L2) but leave more of themselves empty.
-        # Measured on a B200 with 16 / 128, us: 3584 x 3584 rank 16, 16 adapters: 512 rows 9.8 / 12.5,
+        # (The rule does not know how many adapters the rows name: one request's chunk of up to 512 rows takes
+        # the 16-row tiles too, and is slower for it.) Measured on a B200 with 16 / 128, us: 3584 x 3584 rank 16, 16 adapters: 512 rows 9.8 / 12.5,
         # 1024 rows 12.4 / 13.4; 4096 x 6144 rank 64, 16 adapters: 512 rows 19.4 / 23.3, 1024 rows
         # 24.7 / 23.8, one adapter: 256 rows 14.4 / 11.1, 512 rows 20.0 / 12.5, 1024 rows 36.6 / 17.1
         self.tile_rows = 16 if rows <= 512 else 128
@@ -236,7 +243,8 @@ class LoraPlan:
 
 def lora_plan(row_slots: torch.Tensor, slots: int, out: LoraPlan | None = None,
               ws: Workspace | None = None) -> LoraPlan:
-    """Plan of a step from the adapter slot of every row (int32 [M], -1 = no adapter). ``out``: a plan
+    """Plan of a step from the adapter slot of every row (int32 [M], -1 = no adapter), by one CTA (B200, 16 /
+    1024 slots, us: 64 rows 2.5 / 8.8, 2048 rows 3.9 / 11, 8185 rows 8.0 / 18). ``out``: a plan
     of the same size to refill (CUDA graphs). A slot outside [-1, slots) counts as none and records
     SQ_ERR_BOUNDS in the workspace status."""
     m = row_slots.numel()
@@ -269,7 +277,9 @@ def lora_linear(x: torch.Tensor, w: Int4Weight, pool: LoraPool, plan: LoraPlan, 
                 residual: torch.Tensor | None = None, silu_mul: bool = False,
                 ws: Workspace | None = None) -> torch.Tensor:
     """:func:`w4a16_linear` with the rows' adapters added (before the SiLU*up epilogue). The projection
-    (with the residual) is rounded to bf16 before the adapters are added, and their sum again."""
+    (with the residual) is rounded to bf16 before the adapters are added, and their sum again. With
+    ``silu_mul`` that holds for rows without an adapter as well: :func:`w4a16_linear` alone keeps gate and
+    up in fp32, so such a row may differ from it by those roundings."""
     if not silu_mul:
         y = w4a16_linear(x, w, out=out, residual=residual, ws=ws)
         return lora_add(x, pool, plan, y, out=y, ws=ws)
