@@ -77,10 +77,12 @@ def step_layout(ctx_len: torch.Tensor, q_len: torch.Tensor, block_tables: torch.
     the row (``out.totals[1]`` of them in all). A token whose page is -1 (given back) gets slot -1.
 
     What does not fit is not written and records SQ_ERR_BOUNDS in the workspace status: tokens past
-    the buffers, pages past the row's width or the end of the free list (their tokens get slot -1).
+    the buffers, pages past the row's width or the end of the free list (their tokens get slot -1),
+    tiles past ``max_tiles`` (their queries are not computed).
     A sequence whose tokens do not all fit rests: its ``kv_len`` is ``ctx_len`` (at most what its row
     of the table can hold), its ``last_row`` -1, and its tiles are padding, so that attention reads no
-    page that is not the sequence's. A sequence with a length below 0 or of 2^30 tokens and more counts as resting and records it as well. The lengths
+    page that is not the sequence's. A sequence with a length below 0 or of 2^30 tokens and more
+    counts as resting and records it as well. The lengths
     may not be rows of ``out`` itself (copy ``out.kv_len`` to make it the next step's ``ctx_len``), nor
     they or the free list part of the tables."""
     b = ctx_len.numel()
